@@ -23,9 +23,9 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 SOURCES = ["runtime.cu", "gemm_decode.cu", "attn_decode.cu", "ops_small.cu",
            "predictor.cu", "attn_short.cu", "topk_sample.cu", "safetensors.cpp",
            "codec_front.cu", "pf_gemm.cu", "pf_attn.cu",
-           "conv_nlc.cu", "kv_pool.cu"]
+           "conv_nlc.cu", "kv_pool.cu", "rotary.cu", "chunk_attn.cu", "filter_sample.cu"]
 HEADERS = ["tts_common.cuh", "tts_internal.h", "qkrope_row.cuh", "gemm_epilogue.cuh", "pick_rule.cuh",
-           "l2_prefetch.cuh"]
+           "l2_prefetch.cuh", "chunk_batch.cuh"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,5 +1,6 @@
 // C ABI (include/tts_cuda.h) and the native runtime around the kernels: context and scratch
 // ownership, argument checks, the decoder stack, the decode step and its CUDA graph.
+#include <climits>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -300,6 +301,7 @@ tts_status tts_ctx_check(tts_ctx* c, void* stream) {
     if (code & kFlagRopeRange) what += " a position outside the RoPE table, block table or pool;";
     if (code & kFlagSpanRange) what += " an attention span outside 1..max_span or the block table;";
     if (code & kFlagPageRange) what += " a block-table page outside the pool;";
+    if (code & kFlagChunkStarts) what += " chunk row starts that descend or leave the rows;";
     return fail(TTS_ERR_INVALID_ARG, "device data out of range (code " + std::to_string(code) +
                                          "):" + what + " those rows were skipped or read as zero");
   }
@@ -555,6 +557,7 @@ tts_status tts_decode_attention_static_check(void* stream) {
     std::string what;
     if (code & kFlagSpanRange) what += " a span outside 1..max_span or the block table;";
     if (code & kFlagPageRange) what += " a block-table page outside the pool;";
+    if (code & kFlagChunkStarts) what += " chunk row starts that descend or leave the rows;";
     return fail(TTS_ERR_INVALID_ARG, "decode_attention_static: device data out of range (code " +
                                          std::to_string(code) + "):" + what +
                                          " those positions were clamped or read as zero");
@@ -611,6 +614,177 @@ tts_status tts_topk_sample(tts_ctx* c, const float* logits, int rows, int n, con
   return counted(launch_topk_sample(logits, rows, n, n, draws, rows, k, temperature, out, 1,
                                     nullptr, nullptr, 0, nullptr, false, S(stream)),
                  "topk_sample");
+}
+
+tts_status tts_filter_sample(tts_ctx* c, const void* logits, int logits_f16, int rows, int n,
+                             int ldl, const float* draws, const tts_sampling* how, int* out,
+                             void* stream) {
+  if (!c || !logits || !draws || !out)
+    return fail(TTS_ERR_INVALID_ARG, "filter_sample: NULL argument");
+  if (rows < 1 || n < 1 || ldl < 0 || (ldl && ldl < n))
+    return fail(TTS_ERR_INVALID_ARG, "filter_sample: rows, n >= 1 and ldl >= n");
+  if (n > kFilterMaxN)
+    return fail(TTS_ERR_UNSUPPORTED_SHAPE,
+                "filter_sample: n=" + std::to_string(n) + " exceeds 262144");
+  DeviceGuard g(c->device);
+  FilterSampleRequest r;
+  r.logits = logits;
+  r.f16 = logits_f16 != 0;
+  r.rows = rows;
+  r.n = n;
+  r.ldl = ldl ? ldl : n;
+  r.draws = draws;
+  if (how) {
+    r.temperature = how->temperature;
+    r.top_k = how->top_k;
+    r.top_p = how->top_p;
+    r.min_p = how->min_p;
+  }
+  r.out = out;
+  return counted(launch_filter_sample(r, S(stream)), "filter_sample");
+}
+
+// ---------------------------------------------------------------- ragged chunks
+
+static tts_status chunk_ok(const char* op, const tts_chunk_batch* b, const tts_kv_cache* kv) {
+  const std::string name = std::string(op) + ": ";
+  std::string why;
+  if (!b || !b->row_start || !b->spans)
+    return fail(TTS_ERR_INVALID_ARG, name + "chunk batch pointers are NULL");
+  if (b->lanes < 1 || b->rows < 0)
+    return fail(TTS_ERR_INVALID_ARG, name + "lanes must be >= 1 and rows >= 0");
+  if (b->lanes > kChunkMaxLanes)
+    return fail(TTS_ERR_UNSUPPORTED_SHAPE, name + "more than 1024 lanes");
+  if (!kv_ok(kv, &why)) return fail(TTS_ERR_INVALID_ARG, name + why);
+  if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages))
+    return fail(TTS_ERR_INVALID_ARG, name + "pools must be 16-byte aligned");
+  if (long(kv->max_blocks) * kv->block_size > INT_MAX)
+    return fail(TTS_ERR_UNSUPPORTED_SHAPE, name + "more than 2^31 positions per lane");
+  return TTS_OK;
+}
+
+static tts_status rotary_ok(const char* op, int hd, int rope_len, int rotary, int interleaved,
+                            const float* cos_t, const float* sin_t) {
+  const std::string name = std::string(op) + ": ";
+  if (hd < 8 || hd > 256 || hd % 8)
+    return fail(TTS_ERR_UNSUPPORTED_SHAPE, name + "head_dim must be a multiple of 8 up to 256");
+  if (rotary < 8 || rotary > hd || rotary % 8)
+    return fail(TTS_ERR_UNSUPPORTED_SHAPE,
+                name + "rotary_dim must be a multiple of 8 up to head_dim");
+  if (rope_len < 1 || (interleaved != 0 && interleaved != 1))
+    return fail(TTS_ERR_INVALID_ARG, name + "rope_len must be >= 1 and interleaved 0 or 1");
+  if (!aligned16(cos_t) || !aligned16(sin_t))
+    return fail(TTS_ERR_INVALID_ARG, name + "tables must be 16-byte aligned");
+  return TTS_OK;
+}
+
+tts_status tts_rotary(tts_ctx* c, const void* x, int x_f16, int rows, int heads, int head_dim,
+                      int ldx, const int* positions, const float* cos_t, const float* sin_t,
+                      int rope_len, int rotary_dim, int interleaved, void* y, int ldy,
+                      void* stream) {
+  if (!c || !x || !positions || !cos_t || !sin_t || !y)
+    return fail(TTS_ERR_INVALID_ARG, "rotary: NULL argument");
+  tts_status rc = rotary_ok("rotary", head_dim, rope_len, rotary_dim, interleaved, cos_t, sin_t);
+  if (rc != TTS_OK) return rc;
+  if (rows < 0 || heads < 1 || long(heads) * head_dim > INT_MAX)
+    return fail(TTS_ERR_INVALID_ARG, "rotary: rows >= 0 and heads >= 1");
+  const int width = heads * head_dim;
+  if (ldx == 0) ldx = width;
+  if (ldy == 0) ldy = width;
+  if (ldx < width || ldy < width || ldx % 8 || ldy % 8 || (x == y && ldx != ldy))
+    return fail(TTS_ERR_INVALID_ARG,
+                "rotary: row strides must be multiples of 8, cover the heads and agree in place");
+  if (!aligned16(x) || !aligned16(y))
+    return fail(TTS_ERR_INVALID_ARG, "rotary: pointers must be 16-byte aligned");
+  if (rows == 0) return TTS_OK;
+  DeviceGuard g(c->device);
+  return counted(launch_rotary(x, x_f16 != 0, rows, heads, head_dim, ldx, positions, cos_t, sin_t,
+                               rope_len, rotary_dim, interleaved != 0, y, ldy, c->gemm.err,
+                               S(stream)),
+                 "rotary");
+}
+
+tts_status tts_rotary_append(tts_ctx* c, const void* qkv, int qkv_f16, int heads,
+                             const tts_chunk_batch* b, const float* norms, float eps,
+                             const float* cos_t, const float* sin_t, int rope_len, int rotary_dim,
+                             int interleaved, const tts_kv_cache* kv, void* q_out, int q_f16,
+                             void* stream) {
+  if (!c || !qkv || !cos_t || !sin_t || !q_out)
+    return fail(TTS_ERR_INVALID_ARG, "rotary_append: NULL argument");
+  tts_status rc = chunk_ok("rotary_append", b, kv);
+  if (rc == TTS_OK)
+    rc = rotary_ok("rotary_append", 128, rope_len, rotary_dim, interleaved, cos_t, sin_t);
+  if (rc != TTS_OK) return rc;
+  if (heads < 1) return fail(TTS_ERR_INVALID_ARG, "rotary_append: heads must be >= 1");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(norms))
+    return fail(TTS_ERR_INVALID_ARG, "rotary_append: pointers must be 16-byte aligned");
+  if (b->rows == 0) return TTS_OK;
+  DeviceGuard g(c->device);
+  RotaryAppendRequest r;
+  r.x = qkv;
+  r.x_f16 = qkv_f16 != 0;
+  r.q_f16 = q_f16 != 0;
+  r.lanes = b->lanes;
+  r.rows = b->rows;
+  r.row_start = b->row_start;
+  r.spans = b->spans;
+  r.norms = norms;
+  r.eps = eps;
+  r.cos_t = cos_t;
+  r.sin_t = sin_t;
+  r.rope_len = rope_len;
+  r.rotary = rotary_dim;
+  r.interleaved = interleaved;
+  r.block_table = kv->block_table;
+  r.max_blocks = kv->max_blocks;
+  r.block_size = kv->block_size;
+  r.num_blocks = kv->num_blocks;
+  r.heads = heads;
+  r.n_kv = kv->n_kv;
+  r.k_pool = static_cast<__half*>(kv->k_pages);
+  r.v_pool = static_cast<__half*>(kv->v_pages);
+  r.q_out = q_out;
+  r.err = c->gemm.err;
+  return counted(launch_rotary_append(r, S(stream)), "rotary_append");
+}
+
+tts_status tts_chunk_attention(tts_ctx* c, const void* q, int q_f16, int gqa,
+                               const tts_chunk_batch* b, const tts_kv_cache* kv, float scale,
+                               int window, void* out_f16, void* stream) {
+  if (!c || !q || !out_f16) return fail(TTS_ERR_INVALID_ARG, "chunk_attention: NULL argument");
+  tts_status rc = chunk_ok("chunk_attention", b, kv);
+  if (rc != TTS_OK) return rc;
+  if (gqa < 1 || gqa > 16)
+    return fail(TTS_ERR_UNSUPPORTED_SHAPE, "chunk_attention: gqa must be in 1..16");
+  if (window < 0 || !std::isfinite(scale))
+    return fail(TTS_ERR_INVALID_ARG, "chunk_attention: window >= 0 and a finite scale");
+  if (kv->block_size % 8 && kv->max_blocks != 1)
+    return fail(TTS_ERR_UNSUPPORTED_SHAPE,
+                "chunk_attention: block_size must be a multiple of 8 (or one page per lane)");
+  if (!aligned16(q) || !aligned16(out_f16))
+    return fail(TTS_ERR_INVALID_ARG, "chunk_attention: pointers must be 16-byte aligned");
+  if (b->rows == 0) return TTS_OK;
+  DeviceGuard g(c->device);
+  ChunkAttnRequest r;
+  r.q = q;
+  r.q_f16 = q_f16 != 0;
+  r.lanes = b->lanes;
+  r.rows = b->rows;
+  r.row_start = b->row_start;
+  r.spans = b->spans;
+  r.block_table = kv->block_table;
+  r.max_blocks = kv->max_blocks;
+  r.block_size = kv->block_size;
+  r.num_blocks = kv->num_blocks;
+  r.n_kv = kv->n_kv;
+  r.gqa = gqa;
+  r.k_pool = static_cast<const __half*>(kv->k_pages);
+  r.v_pool = static_cast<const __half*>(kv->v_pages);
+  r.scale = scale;
+  r.window = window;
+  r.out = static_cast<__half*>(out_f16);
+  r.err = c->gemm.err;
+  return counted(launch_chunk_attn(r, S(stream)), "chunk_attention");
 }
 
 // ---------------------------------------------------------------- codec front

@@ -25,6 +25,7 @@ constexpr int kFlagWaitMask = kFlagGemmWait | kFlagConvWait | kFlagAttnWait;
 constexpr int kFlagRopeRange = 256;   // position outside the RoPE table, block table or pool
 constexpr int kFlagSpanRange = 512;   // attention span outside 1..min(max_span, table)
 constexpr int kFlagPageRange = 1024;  // attention page outside the pool
+constexpr int kFlagChunkStarts = 16384;  // a chunk batch's row starts descend or leave its rows
 
 // ------------------------------------------------------------------ device properties
 int num_sms(int device);
@@ -277,6 +278,65 @@ cudaError_t launch_topk_sample(const float* logits, int rows, int n, int ldl, co
                                int draw_rows, int k, float temperature, uint32_t* codes,
                                int code_stride, const float* embed32, float* x_next, int dim,
                                int* positions, bool pdl, cudaStream_t st);
+// Rotation of rows at per-row positions (rotary.cu).
+cudaError_t launch_rotary(const void* x, bool f16, int rows, int heads, int hd, int ldx,
+                          const int* positions, const float* cos_t, const float* sin_t,
+                          int rope_len, int rotary, bool interleaved, void* y, int ldy, int* err,
+                          cudaStream_t st);
+// A ragged chunk's rows (chunk_batch.cuh): QK-norm, rotation, q out, K and V into the pages.
+constexpr int kChunkMaxLanes = 1024;
+struct RotaryAppendRequest {
+  const void* x = nullptr;  // [rows][heads + 2 n_kv][128]
+  bool x_f16 = false, q_f16 = false;
+  int lanes = 0, rows = 0;
+  const int* row_start = nullptr;
+  const int* spans = nullptr;
+  const float* norms = nullptr;  // [2][128] or null
+  float eps = 0.f;
+  const float* cos_t = nullptr;
+  const float* sin_t = nullptr;
+  int rope_len = 0, rotary = 0, interleaved = 0;
+  const int* block_table = nullptr;
+  int max_blocks = 0, block_size = 0, num_blocks = 0;
+  int heads = 0, n_kv = 0;
+  __half* k_pool = nullptr;
+  __half* v_pool = nullptr;
+  void* q_out = nullptr;  // [rows][heads][128]
+  int* err = nullptr;
+};
+cudaError_t launch_rotary_append(const RotaryAppendRequest& r, cudaStream_t st);
+// Attention of a ragged chunk over its lanes' pages (chunk_attn.cu).
+struct ChunkAttnRequest {
+  const void* q = nullptr;  // [rows][n_kv * gqa][128]
+  bool q_f16 = false;
+  int lanes = 0, rows = 0;
+  const int* row_start = nullptr;
+  const int* spans = nullptr;
+  const int* block_table = nullptr;
+  int max_blocks = 0, block_size = 0, num_blocks = 0;
+  int n_kv = 0, gqa = 0;
+  const __half* k_pool = nullptr;
+  const __half* v_pool = nullptr;
+  float scale = 1.f;
+  int window = 0;
+  __half* out = nullptr;  // [rows][n_kv * gqa][128]
+  int* err = nullptr;
+};
+cudaError_t launch_chunk_attn(const ChunkAttnRequest& r, cudaStream_t st);
+// The filtered draw (filter_sample.cu); the per-row settings may be null.
+constexpr int kFilterMaxN = 262144;
+struct FilterSampleRequest {
+  const void* logits = nullptr;  // [rows][ldl]
+  bool f16 = false;
+  int rows = 0, n = 0, ldl = 0;
+  const float* draws = nullptr;
+  const float* temperature = nullptr;
+  const int* top_k = nullptr;
+  const float* top_p = nullptr;
+  const float* min_p = nullptr;
+  int* out = nullptr;
+};
+cudaError_t launch_filter_sample(const FilterSampleRequest& r, cudaStream_t st);
 cudaError_t launch_cast_f32_f16(const float* x, __half* y, long n, cudaStream_t st);
 // Prefill as decode rows (map[r] = (lane, offset)): per-row block-table copies and positions;
 // then each lane's position advanced by its row count.

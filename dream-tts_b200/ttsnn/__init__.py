@@ -16,8 +16,9 @@ from ._ctx import check, ctx, ctx_of, launch_count, ptr, stream
 from ._lib import TtsError
 from . import attn, fused, nlc, qkrope, topk  # noqa: F401  (submodules mirror tts-nn's)
 
-__all__ = ["Proj", "pack_weight", "interleave_gate_up", "rms_norm", "rope_table_f32", "abs_and_rel", "TtsError", "check", "ctx",
-           "launch_count", "attn", "fused", "nlc", "qkrope", "topk"]
+__all__ = ["Proj", "pack_weight", "interleave_gate_up", "rms_norm", "rope_table_f32",
+           "rope_table_scaled", "abs_and_rel", "TtsError", "check", "ctx", "launch_count",
+           "attn", "fused", "nlc", "qkrope", "topk"]
 
 
 class Proj:
@@ -140,6 +141,51 @@ def rope_table_f32(length: int, head_dim: int, base: float,
     ph = t * freq[None, :]
     return (torch.cos(ph).to(torch.float32).to(device),
             torch.sin(ph).to(torch.float32).to(device))
+
+
+def rope_table_scaled(length: int, rotary_dim: int, base: float, kind: str = "linear",
+                      factor: float = 1.0, original: int | None = None, beta_fast: float = 32.0,
+                      beta_slow: float = 1.0, mscale: float | None = None,
+                      device: torch.device | str = "cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """Rotary tables `[length, rotary_dim/2]` for a context `factor` times the trained one
+    (phases in f64, rounded to f32; for `qkrope.rotary` and `qkrope.rotary_append`):
+
+    - "linear": every position divided by `factor` (position interpolation);
+    - "ntk": the base raised to base * factor^(r / (r - 2)), which keeps the fastest pair and
+      divides the slowest one's frequency by `factor`;
+    - "yarn" (Peng et al. 2023, "YaRN"): pairs that turn more than `beta_fast` times in the
+      `original` trained positions are kept, those that turn less than `beta_slow` times are
+      divided by `factor`, a linear ramp over the pair index between; cos and sin are both
+      multiplied by `mscale` (None: 0.1 ln(factor) + 1).
+    """
+    r = int(rotary_dim)
+    if length < 1 or r < 2 or r % 2 or not base > 0 or not factor > 0:
+        raise ValueError("rope_table_scaled: length >= 1, an even rotary_dim, base and factor > 0")
+    i = torch.arange(r // 2, dtype=torch.float64)
+    t = torch.arange(length, dtype=torch.float64)[:, None]
+    scale = 1.0
+    if kind == "linear":
+        freq = base ** (-2.0 * i / r) / factor
+    elif kind == "ntk":
+        if r < 4:
+            raise ValueError("rope_table_scaled: ntk needs rotary_dim >= 4")
+        freq = (base * factor ** (r / (r - 2))) ** (-2.0 * i / r)
+    elif kind == "yarn":
+        if original is None or original < 1 or not beta_fast > beta_slow > 0 or not base > 1:
+            raise ValueError("rope_table_scaled: yarn needs `original` >= 1, base > 1 and "
+                             "beta_fast > beta_slow > 0")
+        freq = base ** (-2.0 * i / r)
+        pair = lambda turns: r * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low = max(math.floor(pair(beta_fast)), 0)
+        high = min(math.ceil(pair(beta_slow)), r - 1)
+        ramp = ((i - low) / max(high - low, 1e-3)).clamp(0, 1)
+        freq = freq * (1 - ramp) + freq / factor * ramp
+        scale = mscale if mscale is not None else (0.1 * math.log(factor) + 1 if factor > 1 else 1.0)
+    else:
+        raise ValueError(f"rope_table_scaled: unknown kind {kind!r}")
+    ph = t * freq[None, :]
+    return ((torch.cos(ph) * scale).to(torch.float32).to(device),
+            (torch.sin(ph) * scale).to(torch.float32).to(device))
 
 
 def abs_and_rel(a: torch.Tensor, b: torch.Tensor) -> tuple[float, float]:

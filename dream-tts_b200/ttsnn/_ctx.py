@@ -31,6 +31,11 @@ def stream() -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def stream_of(t: torch.Tensor) -> int:
+    """The current stream of the tensor's device (which need not be the current device)."""
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
 def ptr(t: torch.Tensor | None) -> C.c_void_p:
     return C.c_void_p(0 if t is None else t.data_ptr())
 

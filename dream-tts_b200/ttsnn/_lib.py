@@ -73,6 +73,16 @@ class TextFeed(C.Structure):
                 ("frames", C.c_void_p)]
 
 
+class ChunkBatch(C.Structure):
+    _fields_ = [("lanes", C.c_int), ("rows", C.c_int), ("row_start", C.c_void_p),
+                ("spans", C.c_void_p)]
+
+
+class Sampling(C.Structure):
+    _fields_ = [("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+                ("min_p", C.c_void_p)]
+
+
 class TensorView(C.Structure):
     _fields_ = [("name", C.c_char_p), ("dtype", C.c_int), ("ndim", C.c_int),
                 ("shape", C.c_longlong * 8), ("data", C.c_void_p), ("nbytes", C.c_size_t)]
@@ -122,6 +132,11 @@ SIGNATURES = {
     "tts_stack_set_pick": [P, C.POINTER(PickRule)],
     "tts_talker_pick": [P, P, I, I, C.POINTER(PickRule), I, P, P],
     "tts_topk_sample": [P, P, I, I, P, I, F, P, P],
+    "tts_filter_sample": [P, P, I, I, I, I, P, C.POINTER(Sampling), P, P],
+    "tts_rotary": [P, P, I, I, I, I, I, P, P, P, I, I, I, P, I, P],
+    "tts_rotary_append": [P, P, I, I, C.POINTER(ChunkBatch), P, F, P, P, I, I, I,
+                          C.POINTER(KvCache), P, I, P],
+    "tts_chunk_attention": [P, P, I, I, C.POINTER(ChunkBatch), C.POINTER(KvCache), F, I, P, P],
     "tts_predictor_set_sampling": [P, P, I, I, F],
     "tts_stack_prefill": [P, C.POINTER(DecodeState), P, P, P, P],
     "tts_rvq_gather": [P, P, I, I, I, I, P, I, I, P, P],

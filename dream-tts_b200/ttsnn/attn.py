@@ -6,8 +6,8 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from ._ctx import ctx_of, ptr, stream
-from .qkrope import contiguous_cache
+from ._ctx import ctx_of, ptr, stream, stream_of
+from .qkrope import chunk_batch, contiguous_cache, same_device
 
 
 def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, span: int,
@@ -39,4 +39,48 @@ def decode_attention_paged(q: torch.Tensor, kv: L.KvCache, spans: torch.Tensor, 
                       dtype=torch.float16 if out_f16 else torch.float32)
     L.call("tts_decode_attention", ctx_of(q), ptr(q), lanes, gqa, C.byref(kv), ptr(spans),
            int(max_span), int(window), ptr(out), 1 if out_f16 else 0, stream())
+    return out
+
+
+def paged_cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> L.KvCache:
+    """One layer's pools `[pages, n_kv, block_size, 128]` f16 and block table int32
+    `[lanes, max_blocks]` as the cache the paged calls take (it keeps the tensors alive)."""
+    if k.shape != v.shape or k.dim() != 4 or k.dtype != torch.float16 or v.dtype != torch.float16:
+        raise ValueError("paged_cache: k and v must be f16 [pages, n_kv, block_size, 128]")
+    if table.dim() != 2 or table.dtype != torch.int32:
+        raise ValueError("paged_cache: the block table must be int32 [lanes, max_blocks]")
+    if not (k.is_contiguous() and v.is_contiguous() and table.is_contiguous()):
+        raise ValueError("paged_cache: pools and table must be contiguous")
+    same_device("paged_cache", k, v, table)
+    pages, n_kv, bs, hd = k.shape
+    kv = L.KvCache(k.data_ptr(), v.data_ptr(), table.data_ptr(), table.shape[1], bs, pages, n_kv, hd)
+    kv.lanes, kv.keep = table.shape[0], (k, v, table)
+    return kv
+
+
+def chunk_attention(q: torch.Tensor, row_start: torch.Tensor, spans: torch.Tensor,
+                    kv: L.KvCache, scale: float, window: int = 0,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a ragged chunk of new rows over their lanes' pages (their own K and V
+    included, see `qkrope.rotary_append`): q `[rows, heads, 128]` f16 or f32, lane i's rows
+    row_start[i] .. row_start[i + 1] at its last positions before spans[i], each seeing the
+    positions up to its own (at most `window` of them, 0: all). Returns f16
+    `[rows, heads * 128]` (or `out`); rows of no lane are not written."""
+    if q.dim() != 3 or q.shape[2] != 128 or q.dtype not in (torch.float16, torch.float32):
+        raise ValueError("chunk_attention: q must be [rows, heads, 128], f16 or f32")
+    rows, heads, _ = q.shape
+    if heads % kv.n_kv:
+        raise ValueError(f"chunk_attention: {heads} heads over {kv.n_kv} kv heads")
+    same_device("chunk_attention", q, row_start, spans, out)
+    b = chunk_batch("chunk_attention", rows, row_start, spans, kv)
+    if out is None:
+        out = torch.empty(rows, heads * 128, device=q.device, dtype=torch.float16)
+    elif out.numel() != q.numel() or out.dtype != torch.float16 or not out.is_contiguous():
+        raise ValueError("chunk_attention: out must be contiguous f16 [rows, heads * 128]")
+    if rows == 0:
+        return out
+    qc = q.contiguous()
+    L.call("tts_chunk_attention", ctx_of(q), qc.data_ptr(), int(q.dtype == torch.float16),
+           heads // kv.n_kv, C.byref(b), C.byref(kv), float(scale), int(window), out.data_ptr(),
+           stream_of(q))
     return out

@@ -6,7 +6,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from ._ctx import ctx_of, ptr, stream
+from ._ctx import ctx_of, ptr, stream, stream_of
 
 
 def eligible(qkv: torch.Tensor, k_cache: torch.Tensor, head_dim: int) -> bool:
@@ -63,3 +63,97 @@ def apply(qkv: torch.Tensor, norms: torch.Tensor, cos: torch.Tensor, sin: torch.
            ptr(sin.contiguous()), cos.shape[0], ptr(pos), C.byref(kv), float(eps), ptr(q),
            stream())
     return q.reshape(b, heads, 1, hd), None
+
+
+def chunk_batch(op: str, rows: int, row_start: torch.Tensor, spans: torch.Tensor,
+                kv: L.KvCache) -> L.ChunkBatch:
+    """The ragged batch of a chunk call: int32 device tensors `row_start [lanes + 1]` and
+    `spans [lanes]` (tts_chunk_batch)."""
+    lanes = spans.numel()
+    if row_start.dtype != torch.int32 or spans.dtype != torch.int32:
+        raise ValueError(f"{op}: row_start and spans must be int32")
+    if row_start.numel() != lanes + 1 or not (row_start.is_contiguous() and spans.is_contiguous()):
+        raise ValueError(f"{op}: row_start must hold one entry more than spans, both contiguous")
+    if lanes > getattr(kv, "lanes", lanes):
+        raise ValueError(f"{op}: {lanes} lanes over a block table of {kv.lanes}")
+    return L.ChunkBatch(lanes, rows, row_start.data_ptr(), spans.data_ptr())
+
+
+def same_device(op: str, x: torch.Tensor, *others: torch.Tensor | None) -> None:
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{op}: tensors on {x.device} and {t.device}")
+
+
+def _tables(op: str, cos: torch.Tensor, sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    if cos.shape != sin.shape or cos.dim() != 2:
+        raise ValueError(f"{op}: cos and sin must be [positions, rotary_dim / 2] both")
+    return cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous()
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+           interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions on `x [rows, heads, head_dim]` (f32 or f16), row r at `positions[r]`
+    (int32): the first 2 * cos.shape[1] dims of each head in half-split or interleaved pairs, the
+    rest copied. x may be a column block of wider rows. Into `out` (may be x), else a new
+    tensor."""
+    if x.dim() != 3 or x.dtype not in (torch.float32, torch.float16):
+        raise ValueError("rotary: x must be [rows, heads, head_dim], f32 or f16")
+    rows, heads, hd = x.shape
+    if positions.dtype != torch.int32 or positions.numel() != rows or not positions.is_contiguous():
+        raise ValueError("rotary: one contiguous int32 position per row")
+    same_device("rotary", x, positions, cos, sin, out)
+    c, s = _tables("rotary", cos, sin)
+    whole = lambda t: (t.stride(2) == 1 and t.stride(1) == hd and t.stride(0) % 8 == 0
+                       and t.stride(0) >= heads * hd and t.data_ptr() % 16 == 0)
+    if out is None:
+        y = torch.empty(rows, heads, hd, device=x.device, dtype=x.dtype)
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or not whole(out):
+            raise ValueError("rotary: out must have x's shape and type, heads side by side and "
+                             "16-byte aligned rows")
+        y = out
+    if rows == 0:
+        return y
+    xc = x if whole(x) else x.contiguous()
+    L.call("tts_rotary", ctx_of(x), xc.data_ptr(), int(x.dtype == torch.float16), rows, heads, hd,
+           xc.stride(0), positions.data_ptr(), c.data_ptr(), s.data_ptr(), c.shape[0],
+           2 * c.shape[1], int(interleaved), y.data_ptr(), y.stride(0), stream_of(x))
+    return y
+
+
+def rotary_append(qkv: torch.Tensor, heads: int, row_start: torch.Tensor, spans: torch.Tensor,
+                  cos: torch.Tensor, sin: torch.Tensor, kv: L.KvCache, interleaved: bool = False,
+                  norms: torch.Tensor | None = None, eps: float = 1e-6, q_f16: bool = True,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """A ragged chunk's rows `qkv [rows, (heads + 2 n_kv) * 128]` (f32 or f16): the QK-norm if
+    `norms [2, 128]` is given, the rotation at each row's position, K and V into the pages; the
+    rotated q `[rows, heads, 128]` is returned, f16 or f32 (or written to `out`). Lane i's rows
+    are row_start[i] .. row_start[i + 1] and spans[i] the positions it holds once they are in."""
+    if qkv.dim() != 2 or qkv.dtype not in (torch.float32, torch.float16):
+        raise ValueError("rotary_append: qkv must be [rows, width], f32 or f16")
+    rows = qkv.shape[0]
+    if qkv.shape[1] != (heads + 2 * kv.n_kv) * 128:
+        raise ValueError("rotary_append: qkv width does not match heads and cache")
+    if norms is not None and norms.numel() != 256:
+        raise ValueError("rotary_append: norms must be [2, 128]")
+    same_device("rotary_append", qkv, row_start, spans, cos, sin, norms, out)
+    c, s = _tables("rotary_append", cos, sin)
+    b = chunk_batch("rotary_append", rows, row_start, spans, kv)
+    if out is None:
+        q = torch.empty(rows, heads, 128, device=qkv.device,
+                        dtype=torch.float16 if q_f16 else torch.float32)
+    else:
+        if (out.numel() != rows * heads * 128 or not out.is_contiguous()
+                or out.dtype not in (torch.float32, torch.float16)):
+            raise ValueError("rotary_append: out must be contiguous [rows, heads, 128], f32 or f16")
+        q = out
+    if rows == 0:
+        return q
+    x = qkv.contiguous()
+    nm = None if norms is None else norms.to(torch.float32).contiguous()
+    L.call("tts_rotary_append", ctx_of(x), x.data_ptr(), int(x.dtype == torch.float16), int(heads),
+           C.byref(b), ptr(nm), float(eps), c.data_ptr(), s.data_ptr(), c.shape[0],
+           2 * c.shape[1], int(interleaved), C.byref(kv), q.data_ptr(),
+           int(q.dtype == torch.float16), stream_of(x))
+    return q

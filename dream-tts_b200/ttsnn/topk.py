@@ -2,10 +2,12 @@
 with caller-supplied draws (crates/tts-nn/src/topk.rs)."""
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
 from . import _lib as L
-from ._ctx import ctx_of, ptr, stream
+from ._ctx import ctx_of, ptr, stream, stream_of
 
 
 def argmax(logits: torch.Tensor, banned: torch.Tensor | None = None) -> torch.Tensor:
@@ -51,4 +53,42 @@ def sample(logits: torch.Tensor, draws: torch.Tensor, k: int, temperature: float
     out = torch.empty(rows, dtype=torch.int32, device=x.device)
     L.call("tts_topk_sample", ctx_of(x), ptr(x), rows, n, ptr(d), int(k), float(temperature),
            ptr(out), stream())
+    return out
+
+
+def _per_row(v, rows: int, dtype: torch.dtype, device: torch.device, name: str):
+    """A setting for every row: None, one value for all, or a tensor of one per row."""
+    if v is None:
+        return None
+    if not isinstance(v, torch.Tensor):
+        return torch.full((rows,), v, dtype=dtype, device=device)
+    if v.numel() != rows or v.device != device:
+        raise ValueError(f"sample_filtered: {name} must hold one value per row, on {device}")
+    return v.to(dtype).contiguous()
+
+
+def sample_filtered(logits: torch.Tensor, draws: torch.Tensor, temperature=None, top_k=None,
+                    top_p=None, min_p=None) -> torch.Tensor:
+    """One id per row of `logits [rows, n]` (f32 or f16; any row stride) drawn with
+    `draws[row]` in [0, 1): at `temperature` (None: 1; 0: the largest logit), from the `top_k`
+    largest (0: all), of those the shortest prefix with a share `top_p` of the weight, of those
+    the ids at least `min_p` times as likely as the first. Each setting is one number or a tensor
+    of one per row. int32 [rows], -1 where no id can be picked (tts_filter_sample)."""
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.float16):
+        raise ValueError("sample_filtered: logits must be [rows, n], f32 or f16")
+    x = logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+    rows, n = x.shape
+    d = _per_row(draws, rows, torch.float32, x.device, "draws")
+    if d is None:
+        raise ValueError("sample_filtered: draws are needed")
+    each = (_per_row(temperature, rows, torch.float32, x.device, "temperature"),
+            _per_row(top_k, rows, torch.int32, x.device, "top_k"),
+            _per_row(top_p, rows, torch.float32, x.device, "top_p"),
+            _per_row(min_p, rows, torch.float32, x.device, "min_p"))
+    how = L.Sampling(*(None if t is None else t.data_ptr() for t in each))
+    out = torch.empty(rows, dtype=torch.int32, device=x.device)
+    if rows == 0:
+        return out
+    L.call("tts_filter_sample", ctx_of(x), x.data_ptr(), int(x.dtype == torch.float16), rows, n,
+           x.stride(0), d.data_ptr(), C.byref(how), out.data_ptr(), stream_of(x))
     return out

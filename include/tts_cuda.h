@@ -227,6 +227,80 @@ TTS_API tts_status tts_topk_sample(tts_ctx* ctx, const float* logits, int rows, 
                                    const float* draws, int k, float temperature,
                                    unsigned int* out, void* stream);
 
+/* The filtered draw of each row's next id (no counterpart in the reference, whose samplers are
+ * tts_topk_sample's and the host's, crates/qwen3tts/src/talker.rs:154-236). logits f32 or f16
+ * [rows][n], `ldl` elements from row to row (0: n), n <= 262144; draws f32 [rows] in [0, 1).
+ * Ids go by logit, larger first, ties by lowest id; w = exp((logit - largest) / temperature).
+ * top_k keeps the first k of them; top_p of those the shortest prefix whose weight reaches top_p
+ * of theirs (at least one id); min_p of those the ids with w >= min_p; the pick is the first id
+ * at which the running weight reaches the draw times the weight of what is kept (the walk of
+ * tts_topk_sample). Weights and sums are held in 64 bits. out i32 [rows]: the pick, or -1 where no
+ * id can be picked. Logits of -inf or NaN are never picked; ids at +inf share the draw.
+ * `how` (NULL: none of it) gives every row its own settings, f32/i32 [rows] on the device, each
+ * nullable: temperature (NULL: 1; <= 0 or NaN: the largest logit's lowest id), top_k (<= 0 or
+ * >= n: off), top_p (>= 1 or NaN: off), min_p (<= 0 or NaN: off, above 1 as 1). Rows need no
+ * alignment beyond their element's. */
+typedef struct tts_sampling {
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+} tts_sampling;
+TTS_API tts_status tts_filter_sample(tts_ctx* ctx, const void* logits, int logits_f16, int rows,
+                                     int n, int ldl, const float* draws, const tts_sampling* how,
+                                     int* out, void* stream);
+
+/* ---------------------------------------------------------------- ragged chunks
+ * New rows of several lanes at once over a paged cache: chunks of long prompts, lanes of one
+ * token each, or both together. Lane i's rows are row_start[i] .. row_start[i + 1] - 1 of the
+ * call's row buffers (none is fine) and spans[i] the positions it holds once they are in, so row
+ * j of its n sits at position spans[i] - n + j. Rows outside [row_start[0], row_start[lanes])
+ * are left as they are. row_start int32 [lanes + 1] and spans int32 [lanes] are device memory:
+ * row starts that descend or leave [0, rows] void the whole call (nothing is written), both that
+ * and a span beyond the block table (its lane's rows are skipped) are reported by
+ * tts_ctx_check. lanes <= 1024. No counterpart in the reference, whose Stack::forward takes one
+ * length for the whole batch (crates/qwen3tts/src/qwen3.rs:294-467). */
+typedef struct tts_chunk_batch {
+  int lanes;
+  int rows; /* of the row buffers */
+  const int* row_start;
+  const int* spans;
+} tts_chunk_batch;
+
+/* Rotary positions (candle_nn::rotary_emb, rope and rope_i): rows of x [rows][heads][head_dim],
+ * f32 or f16, `ldx` elements from row to row (0: heads * head_dim), row r at positions[r]
+ * (device), into y of the same type (may be x itself). Pair (a, b) becomes (a cos - b sin,
+ * b cos + a sin); pairs are dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved = 1,
+ * of the first rotary_dim dims of a head, the rest is copied. cos/sin f32
+ * [rope_len][rotary_dim / 2], scaled for long contexts by whoever makes them. head_dim <= 256,
+ * head_dim and rotary_dim multiples of 8, strides too. A position outside the tables skips its
+ * row and is reported by tts_ctx_check. */
+TTS_API tts_status tts_rotary(tts_ctx* ctx, const void* x, int x_f16, int rows, int heads,
+                              int head_dim, int ldx, const int* positions, const float* cos_t,
+                              const float* sin_t, int rope_len, int rotary_dim, int interleaved,
+                              void* y, int ldy, void* stream);
+
+/* tts_qk_rope_append for a ragged chunk: qkv f32 or f16 [rows][(heads + 2 n_kv) * 128]; the
+ * QK-norm when `norms` is given (f32 [2][128], q's then k's weight, over the whole head), then
+ * the rotation of tts_rotary at each row's position; q f32 or f16 [rows][heads][128] out, K and
+ * V (f16) into the pages (any page size). A position outside the tables or a page outside the
+ * pool skips its row and is reported by tts_ctx_check. */
+TTS_API tts_status tts_rotary_append(tts_ctx* ctx, const void* qkv, int qkv_f16, int heads,
+                                     const tts_chunk_batch* batch, const float* norms, float eps,
+                                     const float* cos_t, const float* sin_t, int rope_len,
+                                     int rotary_dim, int interleaved, const tts_kv_cache* kv,
+                                     void* q_out, int q_f16, void* stream);
+
+/* Attention of a ragged chunk over its lanes' pages, its own K and V rows included: the row at
+ * position p sees positions max(0, p + 1 - window) .. p (window 0: 0 .. p), scores q.k * scale.
+ * q f32 or f16 [rows][n_kv * gqa][128], out f16 of the same shape; gqa 1..16; block_size a
+ * multiple of 8 unless max_blocks == 1. A row that sees no position (more new rows than spans
+ * says) is 0, and what the pages hold at positions a row does not see never reaches it. Pages
+ * outside the pool read as zero and are reported by tts_ctx_check. */
+TTS_API tts_status tts_chunk_attention(tts_ctx* ctx, const void* q, int q_f16, int gqa,
+                                       const tts_chunk_batch* batch, const tts_kv_cache* kv,
+                                       float scale, int window, void* out_f16, void* stream);
+
 /* ---------------------------------------------------------------- decoder stack
  * The qwen3 decoder stack (crates/qwen3tts/src/qwen3.rs:15-467): geometry, per-layer weights
  * (caller-owned device memory, referenced not copied) and the decode step at t == 1. */
