@@ -750,7 +750,8 @@ tts_status tts_rotary_append(tts_ctx* c, const void* qkv, int qkv_f16, int heads
 
 tts_status tts_chunk_attention(tts_ctx* c, const void* q, int q_f16, int gqa,
                                const tts_chunk_batch* b, const tts_kv_cache* kv, float scale,
-                               int window, void* out_f16, void* stream) {
+                               int window, void* out_f16, void* workspace,
+                               size_t workspace_bytes, void* stream) {
   if (!c || !q || !out_f16) return fail(TTS_ERR_INVALID_ARG, "chunk_attention: NULL argument");
   tts_status rc = chunk_ok("chunk_attention", b, kv);
   if (rc != TTS_OK) return rc;
@@ -761,9 +762,16 @@ tts_status tts_chunk_attention(tts_ctx* c, const void* q, int q_f16, int gqa,
   if (kv->block_size % 8 && kv->max_blocks != 1)
     return fail(TTS_ERR_UNSUPPORTED_SHAPE,
                 "chunk_attention: block_size must be a multiple of 8 (or one page per lane)");
-  if (!aligned16(q) || !aligned16(out_f16))
+  if (long(kv->num_blocks) * kv->n_kv * kv->block_size > INT_MAX ||
+      long(b->rows) * gqa > INT_MAX - 1024)
+    return fail(TTS_ERR_UNSUPPORTED_SHAPE,
+                "chunk_attention: more than 2^31 pool rows, or rows of one kv head");
+  if (!aligned16(q) || !aligned16(out_f16) || !aligned16(workspace))
     return fail(TTS_ERR_INVALID_ARG, "chunk_attention: pointers must be 16-byte aligned");
   if (b->rows == 0) return TTS_OK;
+  if (!workspace || workspace_bytes < chunk_attn_workspace(c->device))
+    return fail(TTS_ERR_INVALID_ARG,
+                "chunk_attention: the workspace is smaller than tts_chunk_attention_workspace");
   DeviceGuard g(c->device);
   ChunkAttnRequest r;
   r.q = q;
@@ -783,8 +791,15 @@ tts_status tts_chunk_attention(tts_ctx* c, const void* q, int q_f16, int gqa,
   r.scale = scale;
   r.window = window;
   r.out = static_cast<__half*>(out_f16);
+  r.workspace = workspace;
   r.err = c->gemm.err;
-  return counted(launch_chunk_attn(r, S(stream)), "chunk_attention");
+  rc = counted(launch_chunk_attn(r, c->device, S(stream)), "chunk_attention");
+  if (rc == TTS_OK) ++g_launches;  // the join
+  return rc;
+}
+
+size_t tts_chunk_attention_workspace(const tts_ctx* c) {
+  return c ? chunk_attn_workspace(c->device) : 0;
 }
 
 // ---------------------------------------------------------------- codec front

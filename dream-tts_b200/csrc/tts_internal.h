@@ -320,9 +320,11 @@ struct ChunkAttnRequest {
   float scale = 1.f;
   int window = 0;
   __half* out = nullptr;  // [rows][n_kv * gqa][128]
+  void* workspace = nullptr;  // chunk_attn_workspace(device) bytes
   int* err = nullptr;
 };
-cudaError_t launch_chunk_attn(const ChunkAttnRequest& r, cudaStream_t st);
+size_t chunk_attn_workspace(int device);
+cudaError_t launch_chunk_attn(const ChunkAttnRequest& r, int device, cudaStream_t st);  // 2 launches
 // The filtered draw (filter_sample.cu); the per-row settings may be null.
 constexpr int kFilterMaxN = 262144;
 struct FilterSampleRequest {
@@ -363,5 +365,7 @@ cudaError_t launch_conv(const ConvRequest& r, cudaStream_t st, int device, int* 
 bool make_tmap_2d_f16(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer,
                       uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                       bool swizzle128);
+// Rows of 128 f16 as [2 halves][rows][64 columns], 128-byte swizzle.
+bool make_tmap_rows_f16(CUtensorMap* m, const void* ptr, uint64_t rows, uint32_t box_rows);
 
 }  // namespace tts

@@ -136,7 +136,9 @@ SIGNATURES = {
     "tts_rotary": [P, P, I, I, I, I, I, P, P, P, I, I, I, P, I, P],
     "tts_rotary_append": [P, P, I, I, C.POINTER(ChunkBatch), P, F, P, P, I, I, I,
                           C.POINTER(KvCache), P, I, P],
-    "tts_chunk_attention": [P, P, I, I, C.POINTER(ChunkBatch), C.POINTER(KvCache), F, I, P, P],
+    "tts_chunk_attention": [P, P, I, I, C.POINTER(ChunkBatch), C.POINTER(KvCache), F, I, P, P,
+                            C.c_size_t, P],
+    "tts_chunk_attention_workspace": [P],
     "tts_predictor_set_sampling": [P, P, I, I, F],
     "tts_stack_prefill": [P, C.POINTER(DecodeState), P, P, P, P],
     "tts_rvq_gather": [P, P, I, I, I, I, P, I, I, P, P],
@@ -168,7 +170,7 @@ SIGNATURES = {
 }
 _RESTYPE = {"tts_last_error": C.c_char_p, "tts_launch_count": C.c_longlong,
             "tts_safetensors_count": C.c_int, "tts_kv_pool_free_pages": C.c_int,
-            "tts_kv_pool_page_refs": C.c_int}
+            "tts_kv_pool_page_refs": C.c_int, "tts_chunk_attention_workspace": C.c_size_t}
 
 _lib = None
 

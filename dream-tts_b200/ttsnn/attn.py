@@ -80,7 +80,11 @@ def chunk_attention(q: torch.Tensor, row_start: torch.Tensor, spans: torch.Tenso
     if rows == 0:
         return out
     qc = q.contiguous()
-    L.call("tts_chunk_attention", ctx_of(q), qc.data_ptr(), int(q.dtype == torch.float16),
+    c = ctx_of(q)
+    # from torch's allocator, so that calls on several streams or in several graphs have their own
+    size = int(L.load().tts_chunk_attention_workspace(c))
+    work = torch.empty(size, dtype=torch.uint8, device=q.device)
+    L.call("tts_chunk_attention", c, qc.data_ptr(), int(q.dtype == torch.float16),
            heads // kv.n_kv, C.byref(b), C.byref(kv), float(scale), int(window), out.data_ptr(),
-           stream_of(q))
+           work.data_ptr(), size, stream_of(q))
     return out

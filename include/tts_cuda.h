@@ -296,10 +296,15 @@ TTS_API tts_status tts_rotary_append(tts_ctx* ctx, const void* qkv, int qkv_f16,
  * q f32 or f16 [rows][n_kv * gqa][128], out f16 of the same shape; gqa 1..16; block_size a
  * multiple of 8 unless max_blocks == 1. A row that sees no position (more new rows than spans
  * says) is 0, and what the pages hold at positions a row does not see never reaches it. Pages
- * outside the pool read as zero and are reported by tts_ctx_check. */
+ * outside the pool read as zero and are reported by tts_ctx_check. `workspace` (device,
+ * tts_chunk_attention_workspace bytes for any call on the context's device, contents of no
+ * meaning before or after) belongs to the call until it ends on the GPU: calls that may overlap
+ * need one each. */
+TTS_API size_t tts_chunk_attention_workspace(const tts_ctx* ctx);
 TTS_API tts_status tts_chunk_attention(tts_ctx* ctx, const void* q, int q_f16, int gqa,
                                        const tts_chunk_batch* batch, const tts_kv_cache* kv,
-                                       float scale, int window, void* out_f16, void* stream);
+                                       float scale, int window, void* out_f16, void* workspace,
+                                       size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- decoder stack
  * The qwen3 decoder stack (crates/qwen3tts/src/qwen3.rs:15-467): geometry, per-layer weights

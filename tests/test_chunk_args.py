@@ -44,12 +44,14 @@ def lanes(n=2, rows=8, starts=A, spans=A):
     (1, "NULL", dict(kv=kv(k_pages=0))), (1, "aligned", dict(kv=kv(v_pages=A + 8))),
     (2, "multiple of 8", dict(kv=kv(block_size=12))), (2, "2^31", dict(kv=kv(max_blocks=2 ** 30))),
     (1, "aligned", dict(q=A + 2)), (2, "gqa", dict(gqa=0)), (2, "gqa", dict(gqa=17)),
-    (1, "window", dict(window=-1)), (1, "scale", dict(scale=math.inf))])
+    (1, "window", dict(window=-1)), (1, "scale", dict(scale=math.inf)),
+    (2, "pool rows", dict(kv=kv(num_blocks=2 ** 27))), (2, "rows", dict(b=lanes(rows=2 ** 30))),
+    (1, "aligned", dict(work=A + 8)), (1, "workspace", dict(work=0)), (1, "workspace", dict())])
 def test_chunk_attention_refuses(lib, status, text, change):
-    f = dict(q=A, f16=1, gqa=2, b=lanes(), kv=kv(), scale=1.0, window=0, out=A)
+    f = dict(q=A, f16=1, gqa=2, b=lanes(), kv=kv(), scale=1.0, window=0, out=A, work=A)
     f.update(change)
     refused(lib, status, text, "tts_chunk_attention", CTX, f["q"], f["f16"], f["gqa"], f["b"], f["kv"],
-            f["scale"], f["window"], f["out"], None)
+            f["scale"], f["window"], f["out"], f["work"], 1 << 10, None)
 
 
 @pytest.mark.parametrize("status,text,change", [
