@@ -15,14 +15,14 @@
 // chunks both use every SM, and results do not depend on timing.
 //
 // Warps 0-3 and 4-7: one query row a thread through softmax and output, query tiles 0 and 1.
-// Warp 8 loads K and V (TMA, 8 rows x 128 dims a box, so any page of a multiple of 8 rows, or any
-// contiguous lane), warp 9 issues the MMAs, warp 10 walks the work. S and then P (f16, in place)
+// Warps 8 and 11 load K and V (TMA boxes of whole 256-byte rows within a page), warp 9 issues the MMAs, warp 10 walks the work. S and then P (f16, in place)
 // stay in TMEM, O accumulates in TMEM.
 //
-// Softmax in powers of two against a reference r that is the row's maximum so far or up to 2^7
-// below it: w = 2^(c s - r + 8), c = scale log2 e. O is rescaled only when the maximum passes r by
-// more than that, which random scores hardly ever do after the first units. w is at most 2^15 and
-// keeps f16's 11 bits down to 2^-22 of the row's largest; sums are f32.
+// Softmax in powers of two against a reference r: w = 2^(c s - r + 8), c = scale log2 e. r is the
+// largest c s of the row's first unit and stays while the weights of 64 positions add up to no more
+// than f16 holds; only then O and the sum are brought to a new one (random scores hardly ever ask
+// for it after the first units), so no maximum is looked for in most units. Weights keep f16's 11
+// bits down to 2^-22 of r's; sums are f32.
 #include <mutex>
 
 #include "chunk_batch.cuh"
@@ -35,14 +35,64 @@ constexpr int kCaThreads = 384;
 constexpr int kCaTile = 256;  // flat query rows of a work tile
 constexpr int kCaKeys = 128;  // positions of a unit
 constexpr int kCaSegs = 4;    // work descriptors in flight
-constexpr float kCaSlack = 7.f, kCaBias = 8.f;
+constexpr float kCaBias = 8.f, kCaMost = 65504.f;
+constexpr int kCaFirst = 64;  // positions of a unit whose weights the MMAs get first
 
 // 128 rows x 128 f16 for the MMAs: groups of 8 rows, in each two halves of 64 columns, rows of 128
-// bytes with the 128-byte swizzle (what a TMA box of 8 rows x 2 halves x 64 columns writes).
+// bytes with the 128-byte swizzle (what a TMA box of 64 columns x 8 rows x 2 halves x groups writes).
 constexpr int kCaTileBytes = 128 * 256;
 TTS_DEV uint32_t ca_at(int r, int piece) {  // byte offset of 16-byte piece 0..15 of row r
   return uint32_t(r >> 3) * 2048u + uint32_t(piece >> 3) * 1024u + uint32_t(r & 7) * 128u +
          (uint32_t((piece & 7) ^ (r & 7)) << 4);
+}
+
+// The warp's 32 query rows (`rh`: each lane's row of q [rows * heads][128], -1: zeros) into rows
+// r0 .. r0 + 31 of the tile: half a warp a row of f16, a warp a row of f32, which is split into two
+// f16 pieces (22 bits) so that the scores keep f32 queries' precision.
+TTS_DEV uint32_t ca_sign(uint32_t two_halves, int negate) {
+  return negate ? two_halves ^ 0x80008000u : two_halves;
+}
+TTS_DEV void ca_load_q(uint8_t (*tile)[kCaTileBytes], const __half* q, int rh, int r0, int negate) {
+  const int wl = threadIdx.x & 31, sub = wl >> 4, e = wl & 15;
+  uint4 x[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int at = __shfl_sync(0xffffffffu, rh, 2 * k + sub);
+    x[k] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(q + (size_t)at * 128) + e)
+                   : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    *reinterpret_cast<uint4*>(&tile[0][ca_at(r0 + 2 * k + sub, e)]) =
+        make_uint4(ca_sign(x[k].x, negate), ca_sign(x[k].y, negate), ca_sign(x[k].z, negate),
+                   ca_sign(x[k].w, negate));
+}
+TTS_DEV void ca_load_q(uint8_t (*tile)[kCaTileBytes], const float* q, int rh, int r0, int negate) {
+  const int wl = threadIdx.x & 31;
+#pragma unroll
+  for (int k0 = 0; k0 < 32; k0 += 16) {
+    float4 x[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int at = __shfl_sync(0xffffffffu, rh, k0 + k);
+      x[k] = at >= 0 ? __ldg(reinterpret_cast<const float4*>(q + (size_t)at * 128) + wl)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const __half2 h0 = __floats2half2_rn(x[k].x, x[k].y), h1 = __floats2half2_rn(x[k].z, x[k].w);
+      const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+      const __half2 l0 = __floats2half2_rn(x[k].x - b0.x, x[k].y - b0.y),
+                    l1 = __floats2half2_rn(x[k].z - b1.x, x[k].w - b1.y);
+      const uint32_t to = ca_at(r0 + k0 + k, wl >> 1) + (wl & 1) * 8;
+      *reinterpret_cast<uint2*>(&tile[0][to]) =
+          make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&h0), negate),
+                     ca_sign(*reinterpret_cast<const uint32_t*>(&h1), negate));
+      *reinterpret_cast<uint2*>(&tile[1][to]) =
+          make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&l0), negate),
+                     ca_sign(*reinterpret_cast<const uint32_t*>(&l1), negate));
+    }
+  }
 }
 
 // One run of a work tile's units.
@@ -53,17 +103,30 @@ struct CaSeg {
   int begins, ends;   // whether the run has the work tile's first and last unit
 };
 
-template <int kStages, int kParts>  // kParts: f16 pieces a query element is held in
+template <int kK, int kV, int kParts>  // tiles of K and V in flight; f16 pieces of a query element
 struct CaSmem {
-  uint8_t ring[kStages][kCaTileBytes];
+  uint8_t ring[kK + kV][kCaTileBytes];  // K's, then V's
   uint8_t q[2][kParts][kCaTileBytes];
-  uint64_t full[kStages], empty[kStages], q_full[2], s_full[2], p_full[2], o_full[2];
-  uint64_t seg_full[kCaSegs], seg_empty[kCaSegs], tail, drain;
+  uint64_t full[kK + kV], empty[kK + kV], q_full[2], s_full[2], h_full[2], h_done[2], p_full[2], o_full[2];
+  uint64_t seg_full[kCaSegs], seg_empty[kCaSegs], tail, drain, x_full, x_empty;
+  float x_ref[128], x_sum[128];  // the second group's, where one query tile has both groups
   CaSeg seg[kCaSegs];
   int start[4];  // the CTA's first lane, work tile, head and unit
   int count;     // its units
-  int failed;
+  int4 box_row[2][kCaKeys / 32];  // the loaders' boxes: their pool rows, -1 where none is read
   uint32_t tmem;
+};
+
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
+// A softmax thread's query row in a run.
+struct CaRow {
+  int pr, f, pos, lo;  // in the work tile, flat in the lane; its position, the first it sees
+  int rh;              // its row of q and out [rows * heads][128], -1: none
+  bool one, live, work;  // one query tile; a row at all; any in the warp
 };
 
 // What a split work tile's part was, one per CTA for the run it takes over from the CTA before
@@ -77,7 +140,10 @@ struct CaArgs {
   ChunkAttnRequest r;
   float c;      // |scale| log2 e
   int negate;   // scale < 0: the queries change sign
-  int odd;      // one page per lane of any size
+  int box;      // rows of a page that one copy takes
+  int odd;      // one page per lane, of no multiple of 8 rows
+  uint32_t div_m, div_s;  // p / block_size = p * div_m >> 32 + div_s for 0 <= p < 2^31
+  int wide;     // out is 32-byte aligned: whole sectors at a time
   CaPart* parts;
   float* part_data;
 };
@@ -86,6 +152,86 @@ TTS_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// mbar_wait_warp with its bound (about 2 s) on the SM's own clock: the softmax and the MMAs hand
+// over to each other several times a unit, and reading the global timer on each hand-over cost more
+// than the hand-over.
+TTS_DEV bool ca_wait(uint64_t* bar, uint32_t parity, long long limit = 4000000000ll) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    const long long t0 = clock64();
+    do {
+      ok = mbar_try_wait(bar, parity);
+    } while (!ok && clock64() - t0 < limit);
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+// NaN if any of the three is.
+TTS_DEV float max3(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// Two f32 lanes in one instruction.
+TTS_DEV float2 fma2(float2 a, float2 b, float2 c) {
+  float2 y;
+  asm("{\n\t.reg .b64 x, y, z;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return y;
+}
+TTS_DEV float2 add2(float2 a, float2 b) {
+  float2 y;
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(y.x), "=f"(y.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return y;
+}
+// The f16 weights of N scores (-inf: not seen) against `ref`, two to a word, and their sum.
+template <int N>
+TTS_DEV float ca_weights(const uint32_t* v, uint32_t* y, float c, float ref) {
+  const float bias = ref == -INFINITY ? 0.f : kCaBias - ref;
+  const float2 c2 = make_float2(c, c), b2 = make_float2(bias, bias);
+  // batches of 4 pairs, the exponentials of the next on their way while one is summed and packed
+  float2 w[2][4], part[4];
+  const auto start = [&](int b) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 z = fma2(make_float2(__uint_as_float(v[8 * b + 2 * e]),
+                                        __uint_as_float(v[8 * b + 2 * e + 1])), c2, b2);
+      w[b & 1][e] = make_float2(ex2(z.x), ex2(z.y));
+    }
+  };
+  start(0);
+#pragma unroll
+  for (int b = 0; b < N / 8; ++b) {
+    if (b < N / 8 - 1) start(b + 1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 x = w[b & 1][e];
+      part[e] = b == 0 ? x : add2(part[e], x);
+      const __half2 h = __floats2half2_rn(x.x, x.y);
+      y[4 * b + e] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  const float2 s = add2(add2(part[0], part[1]), add2(part[2], part[3]));
+  return s.x + s.y;
+}
+// max(ref, c times the largest of N scores), NaN if a score is.
+template <int N>
+TTS_DEV float ca_max(const uint32_t* v, float c, float ref) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int e = 0; e < N / 2; ++e)
+    m[e % 4] = max3(m[e % 4], __uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+  const float mx = max3(max3(m[0], m[1], m[2]), m[3], m[3]);
+  return max3(ref, mx * c, mx * c);
 }
 
 // 32 columns of the warp's TMEM lanes, without the wait.
@@ -100,6 +246,11 @@ TTS_DEV void tmem_ld32(uint32_t a, uint32_t* r) {
         "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
         "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(a));
+}
+TTS_DEV void st_global_32(void* p, const uint32_t* r) {  // a whole 32-byte sector
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 // Keeps uses of the 32 registers behind the wait that precedes it.
 TTS_DEV void tmem_tie32(uint32_t* r) {
@@ -124,6 +275,10 @@ TTS_DEV void tmem_st16(uint32_t a, const uint32_t* r) {
       "r"(r[15])
       : "memory");
 }
+// A shared-memory descriptor moved by `by` 16-byte units (its low 14 bits; they do not overflow).
+TTS_DEV uint64_t ca_desc(uint64_t d, int by) {
+  return (d & 0xffffffff00000000ull) | uint32_t(uint32_t(d) + by);
+}
 // D += A . B with A (f16 pairs) in TMEM.
 TTS_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -133,11 +288,6 @@ TTS_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc
       "r"(a), "l"(b_desc), "r"(idesc), "r"(acc)
       : "memory");
 }
-// Boxes of the pool seen as [2 halves][rows][64 columns].
-TTS_DEV void ca_load_group(void* dst, const void* map, uint64_t* bar, int row) {
-  tma_load_3d(dst, map, bar, 0, row, 0);
-}
-
 // First unit and number of units of a lane's work tile k (at least one: rows that see nothing are
 // written too).
 TTS_DEV void ca_units(int n, int pos0, int gqa, int window, int k, int* first, int* count) {
@@ -226,87 +376,93 @@ template <typename Smem>
 TTS_DEV void ca_plan(Smem& S, const CaArgs& a) {
   const int t = threadIdx.x, warp = t >> 5, wl = t & 31;
   const ChunkAttnRequest& r = a.r;
-  long long* tot = reinterpret_cast<long long*>(S.ring[0]);  // [lanes]: units before each lane
-  for (int i = warp; i < r.lanes; i += kCaThreads / 32) {
-    const CaLane l = ca_lane(r, i);
+  int* rows = reinterpret_cast<int*>(S.ring[0]);          // [lanes] new rows
+  int* pos0 = rows + kChunkMaxLanes;                      // [lanes] the first one's position
+  long long* tot = reinterpret_cast<long long*>(pos0 + kChunkMaxLanes);  // [lanes] units
+  const auto lane_units = [&](int n, int p, int from, int step) {
     long long u = 0;
-    for (int k = wl; k < ca_tiles(l.n, r.gqa); k += 32) {
+    for (int k = from; k < ca_tiles(n, r.gqa); k += step) {
       int first, count;
-      ca_units(l.n, l.pos0, r.gqa, r.window, k, &first, &count);
+      ca_units(n, p, r.gqa, r.window, k, &first, &count);
       u += count;
     }
+    return u;
+  };
+  for (int i = t; i < r.lanes; i += kCaThreads) {  // a thread a lane, if it has few work tiles
+    const CaLane l = ca_lane(r, i);
+    rows[i] = l.n;
+    pos0[i] = l.pos0;
+    tot[i] = ca_tiles(l.n, r.gqa) <= 4 ? lane_units(l.n, l.pos0, 0, 1) * r.n_kv : -1;
+  }
+  __syncthreads();
+  for (int i = warp; i < r.lanes; i += kCaThreads / 32) {  // a warp a longer one
+    if (tot[i] >= 0) continue;
+    long long u = lane_units(rows[i], pos0[i], wl, 32);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
     if (wl == 0) tot[i] = u * r.n_kv;
   }
   __syncthreads();
   if (warp == 0) {
-    long long all = 0;
-    for (int i0 = 0; i0 < r.lanes; i0 += 32) {
-      const long long mine = i0 + wl < r.lanes ? tot[i0 + wl] : 0;
+    const auto before = [&](long long mine) {  // the sum over lower warp lanes
       long long inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const long long x = __shfl_up_sync(0xffffffffu, inc, o);
         if (wl >= o) inc += x;
       }
-      if (i0 + wl < r.lanes) tot[i0 + wl] = all + inc - mine;
-      all += __shfl_sync(0xffffffffu, inc, 31);
-    }
-    __syncwarp();
+      return inc - mine;
+    };
+    // a warp lane owns a run of lanes
+    const int each = (r.lanes + 31) / 32, l0 = min(r.lanes, wl * each),
+              l1 = min(r.lanes, l0 + each);
+    long long mine = 0;
+    for (int i = l0; i < l1; ++i) mine += tot[i];
+    const long long pre = before(mine);
+    const long long all = __shfl_sync(0xffffffffu, pre + mine, 31);
     const long long per = (all + gridDim.x - 1) / gridDim.x;
     const long long lo = per * blockIdx.x, hi = lo + per < all ? lo + per : all;
     if (wl == 0) S.count = lo < hi ? int(hi - lo) : 0;
     if (lo < hi) {
-      // the last lane that starts at or before `lo` (lanes without rows start where the next does)
-      int lane = 0;
-      for (int i0 = 0; i0 < r.lanes; i0 += 32) {
-        const bool at = i0 + wl < r.lanes && tot[i0 + wl] <= lo;
-        const unsigned m = __ballot_sync(0xffffffffu, at);
-        if (m) lane = i0 + 31 - __clz(m);
+      // the lane that unit `lo` belongs to, and its place there
+      int lane = -1;
+      long long rem = lo - pre;
+      if (rem >= 0 && rem < mine) {
+        lane = l0;
+        while (rem >= tot[lane]) rem -= tot[lane++];
       }
-      long long rem = lo - tot[lane];
-      const CaLane l = ca_lane(r, lane);
-      for (int k0 = 0;; k0 += 32) {
+      const int owner = __ffs(__ballot_sync(0xffffffffu, lane >= 0)) - 1;
+      lane = __shfl_sync(0xffffffffu, lane, owner);
+      rem = __shfl_sync(0xffffffffu, rem, owner);
+      const int n = rows[lane], p = pos0[lane], tiles = ca_tiles(n, r.gqa);
+      for (int k0 = 0; k0 < tiles; k0 += 32) {
         int first = 0, count = 0;
-        if (k0 + wl < ca_tiles(l.n, r.gqa))
-          ca_units(l.n, l.pos0, r.gqa, r.window, k0 + wl, &first, &count);
-        const long long mine = (long long)count * r.n_kv;
-        long long inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-          if (wl >= o) inc += x;
-        }
-        const unsigned m = __ballot_sync(0xffffffffu, rem < inc);
+        if (k0 + wl < tiles) ca_units(n, p, r.gqa, r.window, k0 + wl, &first, &count);
+        const long long here = (long long)count * r.n_kv, low = before(here);
+        const unsigned m = __ballot_sync(0xffffffffu, rem >= low && rem < low + here);
         if (m) {
           if (wl == __ffs(m) - 1) {
-            const int in = int(rem - (inc - mine));
             S.start[0] = lane;
             S.start[1] = k0 + wl;
-            S.start[2] = in / count;
-            S.start[3] = in % count;
+            S.start[2] = int(rem - low) / count;
+            S.start[3] = int(rem - low) % count;
           }
           break;
         }
-        rem -= __shfl_sync(0xffffffffu, inc, 31);
-        if (k0 > ca_tiles(l.n, r.gqa)) {  // not reached: `lo` lies within the lane's units
-          if (wl == 0) S.count = 0;
-          break;
-        }
+        rem -= __shfl_sync(0xffffffffu, low + here, 31);
       }
     }
   }
   __syncthreads();
 }
 
-template <typename TQ, int kStages, int kParts>
+template <typename TQ, int kK, int kV, int kParts>
 __global__ void __launch_bounds__(kCaThreads, 1)
     chunk_attn_kernel(const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ CaArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  typedef CaSmem<kStages, kParts> Smem;
+  typedef CaSmem<kK, kV, kParts> Smem;
   Smem& S = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                      ~uintptr_t(1023));
   const int t = threadIdx.x, warp = t >> 5, wl = t & 31;
@@ -324,23 +480,26 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   ca_plan(S, a);
   if (S.count == 0) return;
   if (t == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kK + kV; ++i) {
       mbar_init(&S.full[i], 1);
       mbar_init(&S.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&S.q_full[i], 4);
       mbar_init(&S.s_full[i], 1);
+      mbar_init(&S.h_full[i], 4);  // half of P
+      mbar_init(&S.h_done[i], 1);
       mbar_init(&S.p_full[i], 4);
       mbar_init(&S.o_full[i], 1);
     }
     for (int i = 0; i < kCaSegs; ++i) {
       mbar_init(&S.seg_full[i], 1);
-      mbar_init(&S.seg_empty[i], 10);
+      mbar_init(&S.seg_empty[i], 11);
     }
+    mbar_init(&S.x_full, 4);
+    mbar_init(&S.x_empty, 4);
     mbar_init(&S.tail, 1);
     mbar_init(&S.drain, 1);
-    S.failed = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -359,7 +518,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   uint32_t seg_phase = 0;
   // every role reads the work in order and frees its slot at once
   const auto next_seg = [&](CaSeg* s) {
-    if (!mbar_wait_warp(&S.seg_full[seg_slot], seg_phase)) return false;
+    if (!ca_wait(&S.seg_full[seg_slot], seg_phase)) return false;
     *s = S.seg[seg_slot];
     __syncwarp();
     if (wl == 0) mbar_arrive(&S.seg_empty[seg_slot]);
@@ -367,7 +526,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     return true;
   };
 
-  if (warp == 10) {
+  // the block's 384 x 168 registers, dealt out by need: 8 warps x 200 + 4 warps x 104
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 10) {
     // ---- the work walk: units in order of lane, work tile, head
     int lane = S.start[0], k = S.start[1], head = S.start[2], off = S.start[3], left = S.count;
     CaLane l = ca_lane(r, lane);
@@ -396,7 +558,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           p.valid = 1;
         }
       }
-      ok = mbar_wait_warp(&S.seg_empty[seg_slot], seg_phase ^ 1);
+      // its queries, which the softmax warps will want in a few microseconds, into L2
+      const int lines = int(sizeof(TQ)) * r.gqa;  // of 128 bytes, per token and kv head
+      const int q0 = s.flat0 / r.gqa, q1 = min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
+      for (int i = wl; i < (q1 - q0) * lines; i += 32)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(
+            static_cast<const char*>(r.q) +
+            (((size_t)(s.row0 + q0 + i / lines) * r.n_kv + s.head) * lines + i % lines) * 128));
+      ok = ca_wait(&S.seg_empty[seg_slot], seg_phase ^ 1);
       if (!ok) break;
       if (wl == 0) {
         S.seg[seg_slot] = s;
@@ -406,332 +575,457 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       if (++seg_slot == kCaSegs) seg_slot = 0, seg_phase ^= 1;
       if (s.units == 0) break;
     }
-  } else if (warp == 8) {
-    // ---- K and V: warp lanes 0-15 a group of 8 K rows each, 16-31 of V rows
-    const int g = wl & 15, is_v = wl >> 4;
-    const CUtensorMap* map = is_v ? &tmV : &tmK;
+  } else if (warp != 9) {
+    // ---- warp 8 K, warp 11 V, by boxes of `box` rows of one page: warp lane g looks up box g, one
+    // elected lane issues them all in one go (a copy then takes it about 50 clocks; one per
+    // reconvergence of the warp took 240)
+    const int v = warp == 11, base = v ? kK : 0, ring = v ? kV : kK;
+    const CUtensorMap* map = v ? &tmV : &tmK;
+    const int boxes = kCaKeys / a.box;
     int slot = 0;
     uint32_t phase = 0, tail_phase = 0;
     CaSeg s;
     while (ok && (ok = next_seg(&s)) && s.units > 0) {
       const int last = min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
       const int hi = s.pos0 + last;  // positions from here on are seen by no row of the tile
-      const auto page_of = [&](int j) {
-        const int p = (s.unit0 + j) * kCaKeys + g * 8;
-        return j < s.units && p < hi
-                   ? r.block_table[(size_t)s.lane * r.max_blocks + p / r.block_size]
-                   : 0;
-      };
-      int page = page_of(0);
+      const int* table = r.block_table + (size_t)s.lane * r.max_blocks;
+      const int end = min(hi, (s.unit0 + s.units) * kCaKeys);
+      // this warp lane's box of the next unit: its position, block and (once read) page
+      int p = s.unit0 * kCaKeys + wl * a.box;
+      const auto block = [&] { return a.odd ? 0 : int(__umulhi(p, a.div_m) >> a.div_s); };
+      int blk = block(), page = wl < boxes && p < end ? table[blk] : -1;
       for (int j = 0; j < s.units; ++j) {
-        const int next = page_of(j + 1);
-        const int p0 = (s.unit0 + j) * kCaKeys, p = p0 + g * 8;
-        const bool seen = p < hi, bad = seen && (page < 0 || page >= r.num_blocks);
-        if (bad) atomicOr(r.err, kFlagPageRange);
-        const int row = (page * r.n_kv + s.head) * r.block_size + p % r.block_size;
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          ok = ok && mbar_wait_warp(&S.empty[slot], phase ^ 1);
-          if (!ok) break;
-          uint8_t* tile = S.ring[slot];
-          const bool mine = is_v == v;
-          const int loads = __popc(__ballot_sync(0xffffffffu, mine && seen && !bad));
-          // groups without a page read as zero; so do V rows that nothing sees, whose stale
-          // bits times a weight of 0 could be NaN
-          const bool tail = v && p0 + kCaKeys > hi;
-          if (mine && (bad || (tail && !seen))) {
-            for (int i = 0; i < 128; ++i)
-              *reinterpret_cast<uint4*>(tile + g * 2048 + i * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async();
-          }
-          __syncwarp();
-          uint64_t* bar = tail ? &S.tail : &S.full[slot];
-          if (wl == 0) mbar_arrive_expect_tx(bar, uint32_t(loads) * 2048u);
-          __syncwarp();
-          if (mine && seen && !bad) ca_load_group(tile + g * 2048, map, bar, row);
-          if (tail) {
-            ok = mbar_wait_warp(&S.tail, tail_phase);
-            tail_phase ^= 1;
-            if (!ok) break;
-            for (int i = wl; i < (8 - (hi & 7)) % 8 * 16 && hi > p0; i += 32)
-              *reinterpret_cast<uint4*>(tile + ca_at(hi - p0 + (i >> 4), i & 15)) =
-                  make_uint4(0, 0, 0, 0);
-            fence_proxy_async();
-            __syncwarp();
-            if (wl == 0) mbar_arrive(&S.full[slot]);
-          }
-          if (++slot == kStages) slot = 0, phase ^= 1;
-        }
-        page = next;
+        const int p0 = (s.unit0 + j) * kCaKeys;
+        const bool seen = wl < boxes && p < hi, bad = seen && (page < 0 || page >= r.num_blocks);
+        const int row =
+            seen && !bad ? (page * r.n_kv + s.head) * r.block_size + (p - blk * r.block_size) : -1;
+        const unsigned load = __ballot_sync(0xffffffffu, row >= 0);
+        const unsigned zero = __ballot_sync(0xffffffffu, bad);
+        p += kCaKeys;
+        blk = block();
+        page = wl < boxes && p < end ? table[blk] : -1;  // on its way while this tile is loaded
+        const bool tail = v && p0 + kCaKeys > hi;
+        uint64_t* full = &S.full[base + slot];
+        ok = ca_wait(&S.empty[base + slot], phase ^ 1);
         if (!ok) break;
+        uint8_t* tile = S.ring[base + slot];
+        if (wl < kCaKeys / 8) reinterpret_cast<int*>(S.box_row[v])[wl] = row;
+        const auto zero_rows = [&](int r0, int n) {
+          for (int e = wl; e < n * 16; e += 32)
+            *reinterpret_cast<uint4*>(tile + ca_at(r0 + (e >> 4), e & 15)) =
+                make_uint4(0, 0, 0, 0);
+        };
+        if (zero) {  // pages outside the pool read as zero
+          if (wl == 0) atomicOr(r.err, kFlagPageRange);
+          for (unsigned m = zero; m; m &= m - 1) zero_rows((__ffs(m) - 1) * a.box, a.box);
+          fence_proxy_async();
+        }
+        __syncwarp();
+        if (elect_one()) {
+          uint64_t* bar = tail ? &S.tail : full;
+          mbar_arrive_expect_tx(bar, uint32_t(__popc(load) * a.box) * 256u);
+          for (int b = 0; b < boxes; b += 4) {
+            const int4 at = S.box_row[v][b >> 2];
+            const auto copy = [&](int i, int from) {
+              uint8_t* dst = tile + (b + i) * a.box * 256;
+              if (from < 0) return;
+              if (a.odd)
+                tma_load_3d(dst, map, bar, 0, from, 0);
+              else
+                tma_load_4d(dst, map, bar, 0, 0, 0, from >> 3);
+            };
+            copy(0, at.x);
+            copy(1, at.y);
+            copy(2, at.z);
+            copy(3, at.w);
+          }
+        }
+        __syncwarp();
+        if (tail) {
+          // rows that nothing sees: their stale bits times a weight of 0 could be NaN
+          ok = ca_wait(&S.tail, tail_phase);
+          tail_phase ^= 1;
+          if (!ok) break;
+          const int keep = max(hi - p0, 0);
+          zero_rows(keep, kCaKeys - keep);
+          fence_proxy_async();
+          __syncwarp();
+          if (wl == 0) mbar_arrive(full);
+        }
+        if (++slot == ring) slot = 0, phase ^= 1;
       }
     }
     if (!ok)  // bounded: copies still on their way
-      for (int i = 0; i < kStages; ++i) mbar_wait(&S.full[i], phase, 100000000ull);
+      for (int i = 0; i < ring; ++i) ca_wait(&S.full[base + i], phase, 200000000ll);
   } else if (warp == 9) {
     // ---- the MMAs. Tile by tile and unit by unit: O_t += P_t.V(j), then S_t = Q_t.K(j + 1) over
     // the P just read (MMAs of one thread run in the order of their issue).
     const uint32_t idesc_s = idesc_f16_f32(128, kCaKeys);
     const uint32_t idesc_o = idesc_f16_f32(128, 128) | (1u << 16);  // B (V) MN-major
-    int slot = 0;
-    uint32_t phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-    const auto advance = [&] {
-      if (++slot == kStages) slot = 0, phase ^= 1;
+    int k_slot = 0, v_slot = 0;
+    uint32_t k_phase = 0, v_phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+    const auto next_k = [&] {
+      if (++k_slot == kK) k_slot = 0, k_phase ^= 1;
     };
-    const auto scores = [&](int tl, int at) {
-      const uint32_t kb = smem_u32(S.ring[at]);
+    // descriptors of the first tiles; others differ in the address alone (in 16 bytes)
+    constexpr int kTile16 = kCaTileBytes / 16;
+    const uint64_t q_desc = smem_desc(smem_u32(S.q), 16, 2048, 2);
+    const uint64_t k_desc = smem_desc(smem_u32(S.ring), 16, 2048, 2);
+    const uint64_t v_desc = smem_desc(smem_u32(S.ring[kK]), 1024, 2048, 2);
+    // S_buf = Q_tl.K^T
+    const auto scores = [&](int buf, int tl, int at) {
+      const uint64_t q = ca_desc(q_desc, tl * kParts * kTile16), k = ca_desc(k_desc, at * kTile16);
 #pragma unroll
-      for (int h = 0; h < kParts; ++h) {
-        const uint32_t qb = smem_u32(S.q[tl][h]);
+      for (int h = 0; h < kParts; ++h)
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
-          const uint32_t o = (kk >> 2) * 1024 + (kk & 3) * 32;
-          umma_f16(tmem + tl * 128, smem_desc(qb + o, 16, 2048, 2), smem_desc(kb + o, 16, 2048, 2),
-                   idesc_s, (h | kk) != 0);
+          constexpr int kHalf16 = 1024 / 16;
+          const int o = (kk >> 2) * kHalf16 + (kk & 3) * 2;
+          umma_f16(tmem + buf * 128, ca_desc(q, h * kTile16 + o), ca_desc(k, o), idesc_s,
+                   (h | kk) != 0);
         }
-      }
-      umma_commit(&S.s_full[tl]);
+      umma_commit(&S.s_full[buf]);
     };
     CaSeg s;
     while (ok && (ok = next_seg(&s)) && s.units > 0) {
-      const int tiles = s.flat0 + 128 < s.n * r.gqa ? 2 : 1;
-      ok = mbar_wait_warp(&S.full[slot], phase);
-      for (int tl = 0; tl < tiles && ok; ++tl) {
-        ok = mbar_wait_warp(&S.q_full[tl], q_phase[tl]);
-        q_phase[tl] ^= 1;
+      // one query tile: units go to the two score buffers in turn, ahead of them the next but one
+      const bool one = s.flat0 + 128 >= s.n * r.gqa;
+      const int ahead = one ? 2 : 1;
+      for (int b = 0; b < 2 && ok; ++b) {
+        if (one && b >= s.units) break;
+        if (b == 0 || one) ok = ca_wait(&S.full[k_slot], k_phase);
+        if (ok && (b == 0 || !one)) {
+          ok = ca_wait(&S.q_full[b], q_phase[b]);
+          q_phase[b] ^= 1;
+        }
         if (!ok) break;
         tc_fence_after();
-        if (elect_one()) scores(tl, slot);
+        if (elect_one()) {
+          scores(b, one ? 0 : b, k_slot);
+          if (one || b == 1) umma_commit(&S.empty[k_slot]);
+        }
         __syncwarp();
+        if (one || b == 1) next_k();
       }
-      if (!ok) break;
-      if (elect_one()) umma_commit(&S.empty[slot]);
-      __syncwarp();
-      advance();
       for (int j = 0; j < s.units && ok; ++j) {
-        const int v_slot = slot;
-        ok = mbar_wait_warp(&S.full[slot], phase);
-        advance();
-        const bool more = j + 1 < s.units;
-        for (int tl = 0; tl < tiles && ok; ++tl) {
-          ok = mbar_wait_warp(&S.p_full[tl], p_phase[tl]);
-          p_phase[tl] ^= 1;
-          if (tl == 0 && more && ok) ok = mbar_wait_warp(&S.full[slot], phase);
+        const bool more = j + ahead < s.units;
+        ok = ca_wait(&S.full[kK + v_slot], v_phase);
+        const uint64_t vd = ca_desc(v_desc, v_slot * kTile16);
+        for (int b = one ? j & 1 : 0; b < (one ? (j & 1) + 1 : 2) && ok; ++b) {
+          const auto values = [&](int kk) {
+            umma_f16_ts(tmem + 256 + b * 128, tmem + b * 128 + kk * 8,
+                        ca_desc(vd, kk * (4096 / 16)), idesc_o, j >= ahead || kk > 0);
+          };
+          ok = ca_wait(&S.h_full[b], p_phase[b]);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t vb = smem_u32(S.ring[v_slot]);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              umma_f16_ts(tmem + 256 + tl * 128, tmem + tl * 128 + kk * 8,
-                          smem_desc(vb + kk * 4096, 1024, 2048, 2), idesc_o, (j | kk) != 0);
+            for (int kk = 0; kk < kCaFirst / 16; ++kk) values(kk);
+            umma_commit(&S.h_done[b]);
+          }
+          __syncwarp();
+          ok = ca_wait(&S.p_full[b], p_phase[b]);
+          p_phase[b] ^= 1;
+          if (ok && more && (b == 0 || one)) ok = ca_wait(&S.full[k_slot], k_phase);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = kCaFirst / 16; kk < 8; ++kk) values(kk);
             if (more)
-              scores(tl, slot);
+              scores(b, one ? 0 : b, k_slot);
             else
-              umma_commit(&S.o_full[tl]);
+              umma_commit(&S.o_full[b]);
           }
           __syncwarp();
         }
         if (!ok) break;
         if (elect_one()) {
-          umma_commit(&S.empty[v_slot]);
-          if (more) umma_commit(&S.empty[slot]);
+          umma_commit(&S.empty[kK + v_slot]);
+          if (more) umma_commit(&S.empty[k_slot]);
         }
         __syncwarp();
-        if (more) advance();
+        if (more) next_k();
+        if (++v_slot == kV) v_slot = 0, v_phase ^= 1;
       }
     }
     if (!ok) {  // bounded: MMAs still running
       if (elect_one()) umma_commit(&S.drain);
       __syncwarp();
-      mbar_wait(&S.drain, 0, 100000000ull);
+      ca_wait(&S.drain, 0, 200000000ll);
     }
-  } else if (warp < 8) {
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---- softmax and output, one query row a thread
     const int tl = warp >> 2, lane_row = t & 127;
     const uint32_t lanes_at = uint32_t((warp & 3) * 32) << 16;
     const uint32_t s_at = tmem + lanes_at + uint32_t(tl * 128);
     const uint32_t o_at = tmem + lanes_at + 256u + uint32_t(tl * 128);
-    uint32_t s_phase = 0, o_phase = 0;
-    CaSeg s;
-    while (ok && (ok = next_seg(&s)) && s.units > 0) {
-      const int f = s.flat0 + tl * 128 + lane_row;
-      if (s.flat0 + tl * 128 >= s.n * r.gqa) continue;  // this query tile has no rows
-      const bool live = f < s.n * r.gqa;
-      const int tok = f / r.gqa;
-      const int head = s.head * r.gqa + f % r.gqa;
-      const int pos = live ? s.pos0 + tok : -1;
-      const int lo = r.window > 0 ? max(0, pos + 1 - r.window) : 0;
-      const bool work = __any_sync(0xffffffffu, live);
-      // the row as f16 pieces in the MMA's layout
-      const uint4* src = reinterpret_cast<const uint4*>(
-          static_cast<const TQ*>(r.q) +
-          ((size_t)(s.row0 + tok) * r.n_kv * r.gqa + head) * 128);
-      constexpr int kWords = int(sizeof(TQ)) / 2;  // 16-byte loads per 8 dims
-#pragma unroll
-      for (int e0 = 0; e0 < 16; e0 += 8) {
-        uint4 x[8 * kWords];
-#pragma unroll
-        for (int i = 0; i < 8 * kWords; ++i)
-          x[i] = live ? __ldg(src + e0 * kWords + i) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          uint4 piece[kParts];
-          __half* h = reinterpret_cast<__half*>(piece);
-          const TQ* v = reinterpret_cast<const TQ*>(x + e * kWords);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float rest = a.negate ? -float(v[i]) : float(v[i]);
-#pragma unroll
-            for (int p = 0; p < kParts; ++p) {
-              h[p * 8 + i] = __float2half_rn(rest);
-              rest -= __half2float(h[p * 8 + i]);
-            }
-          }
-#pragma unroll
-          for (int p = 0; p < kParts; ++p)
-            *reinterpret_cast<uint4*>(&S.q[tl][p][ca_at(lane_row, e0 + e)]) = piece[p];
-        }
-      }
+    uint32_t s_phase = 0, o_phase = 0, x_phase = 0;
+    const auto rows_of = [&](const CaSeg& s) {
+      CaRow w;
+      // one query tile only: its units alternate between the two groups of warps
+      w.one = s.flat0 + 128 >= s.n * r.gqa;
+      w.pr = (w.one ? 0 : tl * 128) + lane_row;
+      w.f = s.flat0 + w.pr;
+      w.live = w.f < s.n * r.gqa;
+      w.work = __any_sync(0xffffffffu, w.live);
+      const int tok = w.f / r.gqa;
+      w.pos = w.live ? s.pos0 + tok : -1;
+      w.lo = r.window > 0 ? max(0, w.pos + 1 - r.window) : 0;
+      w.rh = w.live ? (s.row0 + tok) * (r.n_kv * r.gqa) + s.head * r.gqa + w.f % r.gqa : -1;
+      return w;
+    };
+    const auto load_queries = [&](const CaSeg& s, const CaRow& w) {
+      if (s.units == 0 || (w.one && tl == 1)) return;
+      ca_load_q(S.q[tl], static_cast<const TQ*>(r.q), w.rh, (warp & 3) * 32, a.negate);
       fence_proxy_async();
       tc_fence_before();
       __syncwarp();
       if (wl == 0) mbar_arrive(&S.q_full[tl]);
+    };
+    CaSeg s{};
+    ok = next_seg(&s);
+    CaRow w = rows_of(s);
+    if (ok) load_queries(s, w);
+    while (ok && s.units > 0) {
       // rows of a warp see contiguous ranges: a unit inside all of them needs no mask
-      const int pos_min = __reduce_min_sync(0xffffffffu, live ? pos : INT_MAX);
-      const int lo_max = __reduce_max_sync(0xffffffffu, live ? lo : 0);
-      float ref = -INFINITY, sum = 0.f;
-      for (int j = 0; j < s.units; ++j) {
-        ok = mbar_wait_warp(&S.s_full[tl], s_phase);
+      const int pos_min = __reduce_min_sync(0xffffffffu, w.live ? w.pos : INT_MAX);
+      const int lo_max = __reduce_max_sync(0xffffffffu, w.live ? w.lo : 0);
+      float ref = w.live ? -INFINITY : 0.f, sum = 0.f;
+      bool fresh = true;  // some row has no reference yet
+      const int step0 = w.one ? tl : 0, steps = w.one ? 2 : 1;
+      for (int j = step0; j < s.units; j += steps) {
+        ok = ca_wait(&S.s_full[tl], s_phase);
         s_phase ^= 1;
         if (!ok) break;
         tc_fence_after();
-        if (work) {
-          uint32_t x[4][32];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_ld32(s_at + i * 32, x[i]);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tmem_tie32(x[i]);
+        if (w.work) {
           const int p0 = (s.unit0 + j) * kCaKeys;
-          if (p0 + kCaKeys - 1 > pos_min || p0 < lo_max) {
-            const int first = lo - p0, last = pos - p0;  // columns the row sees
+          const bool edge = p0 + kCaKeys - 1 > pos_min || p0 < lo_max;
+          const int first = w.lo - p0, last = w.pos - p0;  // columns the row sees
+          uint32_t x[kCaKeys];
+          // a part of the unit's positions: their scores in x, their weights over them in TMEM
+          const auto step = [&](auto from, auto to) {
+            constexpr int c0 = decltype(from)::value, n = decltype(to)::value - c0;
+            tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int e = 0; e < n; e += 32) tmem_tie32(x + c0 + e);
+            if (c0 == 0) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (i * 32 + e < first || i * 32 + e > last) x[i][e] = 0xff800000u;  // -inf
-          }
-          float mx = -INFINITY;
+              for (int e = n; e < kCaKeys; e += 32) tmem_ld32(s_at + e, x + e);
+            }
+            if (edge) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+              for (int e = c0; e < c0 + n; ++e)
+                if (e < first || e > last) x[e] = 0xff800000u;  // -inf
+            }
+            float got = 0.f;
+            bool raise = ref == -INFINITY, any = fresh;
+#pragma unroll 1
+            for (int pass = 0; pass < 2; ++pass) {
+              if (any) {
+                // O holds weights against the old reference: bring it, and the sum, to the new one
+                float up = ref;
+                if (raise) {
+                  up = ca_max<n>(x + c0, a.c, ref);
+                  if (up == INFINITY) up = NAN;  // as the row's formula has it
+                }
+                const float keep = up == -INFINITY ? 1.f : ex2(ref - up);
+                ref = up;
+                sum *= keep;
+                fresh = __any_sync(0xffffffffu, ref == -INFINITY);
+                if (c0 > 0) {  // the first part's MMAs; before that, S(j) came after all others
+                  ok = ca_wait(&S.h_done[tl], s_phase ^ 1);
+                  if (!ok) return;
+                  tc_fence_after();
+                }
+                if (j > step0 || c0 > 0) {
+#pragma unroll 1
+                  for (int i = 0; i < 8; ++i) {
+                    float o[16];
+                    uint32_t z[16];
+                    tmem_ld16(o_at + i * 16, o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(x[i][e]));
-          mx *= a.c;
-          const bool up = mx > ref + kCaSlack;
-          if (__any_sync(0xffffffffu, up)) {
-            const float keep = up ? ex2(ref - mx) : 1.f;
-            if (up) ref = mx;
-            sum *= keep;
-            if (j > 0) {  // the MMAs before S(j), O's among them, are complete
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                float o[16];
-                uint32_t y[16];
-                tmem_ld16(o_at + i * 16, o);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(o[e] * keep);
-                tmem_st16(o_at + i * 16, y);
+                    for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(o[e] * keep);
+                    tmem_st16(o_at + i * 16, z);
+                  }
+                }
               }
-            }
-          }
-          const float bias = ref == -INFINITY ? 0.f : kCaBias - ref;
-          float part[4] = {0.f, 0.f, 0.f, 0.f};
+              uint32_t y[n / 2];
+              got = ca_weights<n>(x + c0, y, a.c, ref);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t y[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float w0 = ex2(fmaf(__uint_as_float(x[i][2 * e]), a.c, bias));
-              const float w1 = ex2(fmaf(__uint_as_float(x[i][2 * e + 1]), a.c, bias));
-              part[e & 1] += w0;
-              part[2 + (e & 1)] += w1;
-              const __half2 h = __floats2half2_rn(w0, w1);
-              y[e] = *reinterpret_cast<const uint32_t*>(&h);
+              for (int e = 0; e < n / 2; e += 16) tmem_st16(s_at + c0 / 2 + e, y + e);
+              raise = !(got <= kCaMost) && ref == ref;
+              any = __any_sync(0xffffffffu, raise);
+              if (!any) break;
             }
-            tmem_st16(s_at + i * 16, y);
+            sum += got;
+            tmem_wait_st();
+          };
+#pragma unroll
+          for (int e = 0; e < kCaFirst; e += 32) tmem_ld32(s_at + e, x + e);
+          step(Int<0>(), Int<kCaFirst>());
+          if (ok) {  // the MMAs can start on the first part of P
+            tc_fence_before();
+            __syncwarp();
+            if (wl == 0) mbar_arrive(&S.h_full[tl]);
+            step(Int<kCaFirst>(), Int<kCaKeys>());
           }
-          sum += (part[0] + part[1]) + (part[2] + part[3]);
-          tmem_wait_st();
+          if (!ok) break;
+        } else if (wl == 0) {
+          mbar_arrive(&S.h_full[tl]);
         }
         tc_fence_before();
         __syncwarp();
         if (wl == 0) mbar_arrive(&S.p_full[tl]);
       }
       if (!ok) break;
-      ok = mbar_wait_warp(&S.o_full[tl], o_phase);
-      o_phase ^= 1;
+      // The next run's queries while the last MMAs are on their way: this tile's scores are all
+      // done. (Not where both groups work on one tile, the other's may not be.)
+      CaSeg sn{};
+      ok = next_seg(&sn);
       if (!ok) break;
-      tc_fence_after();
-      if (!work) continue;
-      // ---- out, or the part of a split work tile
-      const bool whole = s.begins && s.ends;
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      __half* dst = r.out + ((size_t)(s.row0 + tok) * r.n_kv * r.gqa + head) * 128;
-      float* part = a.part_data + (size_t)(2 * blockIdx.x + (s.begins ? 1 : 0)) * kCaPartFloats;
-      const int pr = tl * 128 + lane_row;
-      float probe = 0.f;  // NaN once a value is not finite
+      const CaRow wn = rows_of(sn);
+      if (!w.one) load_queries(sn, wn);
+      if (step0 < s.units) {
+        ok = ca_wait(&S.o_full[tl], o_phase);
+        o_phase ^= 1;
+        if (!ok) break;
+        tc_fence_after();
+      }
+      if (w.one && s.units > 1) {
+        // the second group hands over its reference, sum and O, 64 dims at a time, in the place
+        // of the second query tile
+        float* xo = reinterpret_cast<float*>(S.q[1][0]) + lane_row;
+        float mine = 1.f, other = 0.f;  // what the two groups' sums count
+        if (tl == 1) {
+          S.x_ref[lane_row] = ref;
+          S.x_sum[lane_row] = sum;
+        }
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          if (tl == 1) {
+#pragma unroll 1
+            for (int d = 0; d < 64 && w.work; d += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_at + h * 64 + d, o);
+              tmem_wait_ld();
+              tmem_tie32(o);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float o[16];
-        tmem_ld16(o_at + i * 16, o);
+              for (int e = 0; e < 32; ++e) xo[(d + e) * 128] = __uint_as_float(o[e]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (wl == 0) mbar_arrive(&S.x_full);
+            ok = ca_wait(&S.x_empty, x_phase);
+          } else {
+            ok = ca_wait(&S.x_full, x_phase);
+            if (ok && h == 0) {
+              const float ref1 = S.x_ref[lane_row], top = max3(ref, ref1, ref1);
+              mine = ref == -INFINITY ? 0.f : ex2(ref - top);
+              other = ref1 == -INFINITY ? 0.f : ex2(ref1 - top);
+              sum = sum * mine + S.x_sum[lane_row] * other;
+              ref = top;
+            }
+#pragma unroll 1
+            for (int d = 0; d < 64 && w.work && ok; d += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_at + h * 64 + d, o);
+              tmem_wait_ld();
+              tmem_tie32(o);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) probe = fmaf(o[e], 0.f, probe);
-        if (!live) continue;
-        if (whole) {
-          uint4 y[2];
-          __half2* h = reinterpret_cast<__half2*>(y);
+              for (int e = 0; e < 32; ++e)
+                o[e] = __float_as_uint(fmaf(xo[(d + e) * 128], other, __uint_as_float(o[e]) * mine));
+              tmem_st16(o_at + h * 64 + d, o);
+              tmem_st16(o_at + h * 64 + d + 16, o + 16);
+              tmem_wait_st();
+            }
+            __syncwarp();
+            if (wl == 0) mbar_arrive(&S.x_empty);
+          }
+          x_phase ^= 1;
+          if (!ok) break;
+        }
+        if (!ok) break;
+      }
+      if (w.one) load_queries(sn, wn);
+      if (w.work && (!w.one || tl == 0)) {
+        // ---- out, or the part of a split work tile
+        const bool whole = s.begins && s.ends;
+        const float total = ref == -INFINITY ? 0.f : sum;  // 0: the row saw nothing
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        float* part = a.part_data + (size_t)(2 * blockIdx.x + (s.begins ? 1 : 0)) * kCaPartFloats;
+        float probe = 0.f;  // NaN once a value is not finite
+        uint32_t o[2][32];
+        tmem_ld32(o_at, o[0]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] = __floats2half2_rn(o[2 * e] * inv, o[2 * e + 1] * inv);
-          reinterpret_cast<uint4*>(dst)[2 * i] = y[0];
-          reinterpret_cast<uint4*>(dst)[2 * i + 1] = y[1];
-        } else {
+        for (int i = 0; i < 4; ++i) {
+          uint32_t* v = o[i & 1];
+          tmem_wait_ld();
+          tmem_tie32(v);
+          if (i < 3) tmem_ld32(o_at + (i + 1) * 32, o[(i + 1) & 1]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            reinterpret_cast<float4*>(part)[(i * 4 + e) * kCaTile + pr] =
-                make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          for (int e = 0; e < 32; ++e) probe = fmaf(__uint_as_float(v[e]), 0.f, probe);
+          if (!w.live) continue;
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 16) {
+              uint32_t y[8];
+#pragma unroll
+              for (int d = 0; d < 8; ++d) {
+                const __half2 h = __floats2half2_rn(__uint_as_float(v[e + 2 * d]) * inv,
+                                                    __uint_as_float(v[e + 2 * d + 1]) * inv);
+                y[d] = *reinterpret_cast<const uint32_t*>(&h);
+              }
+              __half* to = r.out + (size_t)w.rh * 128 + i * 32 + e;
+              if (a.wide) {
+                st_global_32(to, y);
+              } else {
+                reinterpret_cast<uint4*>(to)[0] = make_uint4(y[0], y[1], y[2], y[3]);
+                reinterpret_cast<uint4*>(to)[1] = make_uint4(y[4], y[5], y[6], y[7]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              reinterpret_cast<uint4*>(part)[(i * 8 + e) * kCaTile + w.pr] =
+                  make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          }
+        }
+        if (!whole && w.live) {
+          part[kCaTile * 128 + w.pr] = ref;
+          part[kCaTile * 129 + w.pr] = total;
+        }
+        unsigned again = __ballot_sync(0xffffffffu, w.live && probe != 0.f);
+        const int hi = s.pos0 + min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
+        while (again) {
+          const int src = __ffs(again) - 1;
+          again &= again - 1;
+          float4 y;
+          const float sref = __shfl_sync(0xffffffffu, ref, src);
+          const float sinv = __shfl_sync(0xffffffffu, inv, src);
+          const int sf = __shfl_sync(0xffffffffu, w.f, src);
+          const int spr = __shfl_sync(0xffffffffu, w.pr, src);
+          const int at = __shfl_sync(0xffffffffu, w.rh, src);
+          if (!ca_repair<TQ>(a, s, sf, hi, sref, &y)) continue;
+          __syncwarp();  // after the row's own stores
+          if (whole) {
+            __half2* h = reinterpret_cast<__half2*>(r.out + (size_t)at * 128 + wl * 4);
+            h[0] = __floats2half2_rn(y.x * sinv, y.y * sinv);
+            h[1] = __floats2half2_rn(y.z * sinv, y.w * sinv);
+          } else {
+            reinterpret_cast<float4*>(part)[wl * kCaTile + spr] = y;
+          }
         }
       }
-      if (!whole && live) {
-        part[kCaTile * 128 + pr] = ref;
-        part[kCaTile * 129 + pr] = sum;
-      }
-      unsigned again = __ballot_sync(0xffffffffu, live && probe != 0.f);
-      const int hi = s.pos0 + min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
-      while (again) {
-        const int src = __ffs(again) - 1;
-        again &= again - 1;
-        float4 o;
-        const float sref = __shfl_sync(0xffffffffu, ref, src);
-        const float sinv = __shfl_sync(0xffffffffu, inv, src);
-        const int sf = __shfl_sync(0xffffffffu, f, src), spr = __shfl_sync(0xffffffffu, pr, src);
-        if (!ca_repair<TQ>(a, s, sf, hi, sref, &o)) continue;
-        if (whole) {
-          __half2* h = reinterpret_cast<__half2*>(
-              r.out + ((size_t)(s.row0 + sf / r.gqa) * r.n_kv * r.gqa + s.head * r.gqa +
-                       sf % r.gqa) * 128 + wl * 4);
-          h[0] = __floats2half2_rn(o.x * sinv, o.y * sinv);
-          h[1] = __floats2half2_rn(o.z * sinv, o.w * sinv);
-        } else {
-          reinterpret_cast<float4*>(part)[wl * kCaTile + spr] = o;
-        }
-      }
+      s = sn;
+      w = wn;
     }
   }
-  if (!ok && wl == 0) {
-    atomicOr(r.err, kFlagAttnWait);
-    S.failed = 1;
-  }
+  if (!ok && wl == 0) atomicOr(r.err, kFlagAttnWait);
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
@@ -795,10 +1089,11 @@ size_t chunk_attn_workspace(int device) {
   return size_t(num_sms(device)) * 2 * (sizeof(CaPart) + sizeof(float) * kCaPartFloats);
 }
 
-template <typename TQ, int kStages, int kParts>
+template <typename TQ, int kK, int kV, int kParts>
 static cudaError_t launch_as(const CUtensorMap& k, const CUtensorMap& v, const CaArgs& a, int ctas,
                              int device, cudaStream_t st) {
-  const size_t smem = sizeof(CaSmem<kStages, kParts>) + 1024;
+  constexpr size_t smem = sizeof(CaSmem<kK, kV, kParts>) + 1024;
+  static_assert(smem <= 232448, "227 KB a block");
   {
     // the opt-in shared-memory limit is a per-device function attribute
     static std::mutex mu;
@@ -806,33 +1101,48 @@ static cudaError_t launch_as(const CUtensorMap& k, const CUtensorMap& v, const C
     std::lock_guard<std::mutex> lock(mu);
     if (device >= 0 && device < 64 && !done[device]) {
       const cudaError_t e =
-          cudaFuncSetAttribute(chunk_attn_kernel<TQ, kStages, kParts>,
+          cudaFuncSetAttribute(chunk_attn_kernel<TQ, kK, kV, kParts>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
       if (e != cudaSuccess) return e;
       done[device] = true;
     }
   }
-  chunk_attn_kernel<TQ, kStages, kParts><<<ctas, kCaThreads, smem, st>>>(k, v, a);
+  chunk_attn_kernel<TQ, kK, kV, kParts><<<ctas, kCaThreads, smem, st>>>(k, v, a);
   return cudaGetLastError();
 }
 
 cudaError_t launch_chunk_attn(const ChunkAttnRequest& r, int device, cudaStream_t st) {
   const uint64_t rows = uint64_t(r.num_blocks) * r.n_kv * r.block_size;
   CUtensorMap tmK, tmV;
-  if (!make_tmap_rows_f16(&tmK, r.k_pool, rows, 8) || !make_tmap_rows_f16(&tmV, r.v_pool, rows, 8)) {
+  // a copy never leaves its page: the largest power of two that divides the page, 8 rows where
+  // only the whole lane is contiguous
+  const bool odd = r.block_size % 8 != 0;
+  int box = 8;
+  while (!odd && box < kCaKeys && r.block_size % (2 * box) == 0) box *= 2;
+  if (!make_tmap_rows_f16(&tmK, r.k_pool, rows, box, odd) ||
+      !make_tmap_rows_f16(&tmV, r.v_pool, rows, box, odd)) {
     set_error("chunk_attention: cuTensorMapEncodeTiled failed (pools must be 16-byte aligned)");
     return cudaErrorInvalidValue;
   }
   const int ctas = num_sms(device);
   CaArgs a{};
   a.r = r;
+  a.box = box;
+  a.odd = odd;
+  a.wide = (reinterpret_cast<uintptr_t>(r.out) & 31) == 0;
+  // for a divisor of 8 or more and dividends of 31 bits: m = floor(2^(31 + l) / d) + 1 with
+  // l = ceil(log2 d) is exact (Granlund and Montgomery 1994)
+  int l = 3;
+  while ((1ll << l) < r.block_size) ++l;
+  a.div_m = uint32_t((1ull << (31 + l)) / uint32_t(r.block_size) + 1);
+  a.div_s = l - 1;
   a.negate = r.scale < 0.f;
   // a scale of 0 still has to keep masked scores at -infinity
   a.c = fmaxf(fabsf(r.scale) * 1.4426950408889634f, 1e-30f);
   a.parts = static_cast<CaPart*>(r.workspace);
   a.part_data = reinterpret_cast<float*>(a.parts + 2 * ctas);
-  cudaError_t e = r.q_f16 ? launch_as<__half, 5, 1>(tmK, tmV, a, ctas, device, st)
-                          : launch_as<float, 3, 2>(tmK, tmV, a, ctas, device, st);
+  cudaError_t e = r.q_f16 ? launch_as<__half, 3, 2, 1>(tmK, tmV, a, ctas, device, st)
+                          : launch_as<float, 2, 1, 2>(tmK, tmV, a, ctas, device, st);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas, kCaTile / 32, 1);

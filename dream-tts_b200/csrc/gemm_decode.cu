@@ -691,15 +691,17 @@ bool make_tmap_2d_f16(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t 
   return r == CUDA_SUCCESS;
 }
 
-bool make_tmap_rows_f16(CUtensorMap* m, const void* ptr, uint64_t rows, uint32_t box_rows) {
+bool make_tmap_rows_f16(CUtensorMap* m, const void* ptr, uint64_t rows, uint32_t box_rows,
+                        bool any_row) {
   auto fn = encode_fn();
   if (!fn) return false;
-  cuuint64_t dims[3] = {64, rows, 2};
-  cuuint64_t strides[2] = {256, 128};
-  cuuint32_t box[3] = {64, box_rows, 2};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(ptr), dims, strides,
-                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  // any_row: [2 halves][rows][64], boxes of 8 rows; else [rows / 8][2 halves][8][64]
+  cuuint64_t dims[4] = {64, any_row ? rows : 8, 2, rows / 8};
+  cuuint64_t strides[3] = {256, 128, 2048};
+  cuuint32_t box[4] = {64, 8, 2, box_rows / 8};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, any_row ? 3 : 4, const_cast<void*>(ptr), dims,
+                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS;
 }

@@ -658,7 +658,7 @@ static tts_status chunk_ok(const char* op, const tts_chunk_batch* b, const tts_k
   if (!kv_ok(kv, &why)) return fail(TTS_ERR_INVALID_ARG, name + why);
   if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages))
     return fail(TTS_ERR_INVALID_ARG, name + "pools must be 16-byte aligned");
-  if (long(kv->max_blocks) * kv->block_size > INT_MAX)
+  if (long(kv->max_blocks) * kv->block_size > INT_MAX - 1024)
     return fail(TTS_ERR_UNSUPPORTED_SHAPE, name + "more than 2^31 positions per lane");
   return TTS_OK;
 }
@@ -763,9 +763,9 @@ tts_status tts_chunk_attention(tts_ctx* c, const void* q, int q_f16, int gqa,
     return fail(TTS_ERR_UNSUPPORTED_SHAPE,
                 "chunk_attention: block_size must be a multiple of 8 (or one page per lane)");
   if (long(kv->num_blocks) * kv->n_kv * kv->block_size > INT_MAX ||
-      long(b->rows) * gqa > INT_MAX - 1024)
+      long(b->rows) * gqa * kv->n_kv > INT_MAX - 1024)
     return fail(TTS_ERR_UNSUPPORTED_SHAPE,
-                "chunk_attention: more than 2^31 pool rows, or rows of one kv head");
+                "chunk_attention: more than 2^31 pool rows, or query rows");
   if (!aligned16(q) || !aligned16(out_f16) || !aligned16(workspace))
     return fail(TTS_ERR_INVALID_ARG, "chunk_attention: pointers must be 16-byte aligned");
   if (b->rows == 0) return TTS_OK;

@@ -365,7 +365,10 @@ cudaError_t launch_conv(const ConvRequest& r, cudaStream_t st, int device, int* 
 bool make_tmap_2d_f16(CUtensorMap* m, const void* ptr, uint64_t inner, uint64_t outer,
                       uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                       bool swizzle128);
-// Rows of 128 f16 as [2 halves][rows][64 columns], 128-byte swizzle.
-bool make_tmap_rows_f16(CUtensorMap* m, const void* ptr, uint64_t rows, uint32_t box_rows);
+// Rows of 128 f16 into groups of [2 halves][8 rows][64 columns], 128-byte swizzle: boxes of
+// box_rows from any multiple of 8 (4 coordinates: 0, 0, 0, row / 8), or with any_row of 8 rows from
+// any row (3 coordinates: 0, row, 0).
+bool make_tmap_rows_f16(CUtensorMap* m, const void* ptr, uint64_t rows, uint32_t box_rows,
+                        bool any_row);
 
 }  // namespace tts

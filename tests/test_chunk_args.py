@@ -45,7 +45,7 @@ def lanes(n=2, rows=8, starts=A, spans=A):
     (2, "multiple of 8", dict(kv=kv(block_size=12))), (2, "2^31", dict(kv=kv(max_blocks=2 ** 30))),
     (1, "aligned", dict(q=A + 2)), (2, "gqa", dict(gqa=0)), (2, "gqa", dict(gqa=17)),
     (1, "window", dict(window=-1)), (1, "scale", dict(scale=math.inf)),
-    (2, "pool rows", dict(kv=kv(num_blocks=2 ** 27))), (2, "rows", dict(b=lanes(rows=2 ** 30))),
+    (2, "pool rows", dict(kv=kv(num_blocks=2 ** 27))), (2, "rows", dict(b=lanes(rows=2 ** 29))),
     (1, "aligned", dict(work=A + 8)), (1, "workspace", dict(work=0)), (1, "workspace", dict())])
 def test_chunk_attention_refuses(lib, status, text, change):
     f = dict(q=A, f16=1, gqa=2, b=lanes(), kv=kv(), scale=1.0, window=0, out=A, work=A)
