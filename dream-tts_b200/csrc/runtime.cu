@@ -621,8 +621,8 @@ tts_status tts_filter_sample(tts_ctx* c, const void* logits, int logits_f16, int
                              void* stream) {
   if (!c || !logits || !draws || !out)
     return fail(TTS_ERR_INVALID_ARG, "filter_sample: NULL argument");
-  if (rows < 1 || n < 1 || ldl < 0 || (ldl && ldl < n))
-    return fail(TTS_ERR_INVALID_ARG, "filter_sample: rows, n >= 1 and ldl >= n");
+  if (rows < 1 || n < 1 || ldl < 0 || (ldl && ldl < n) || rows > INT_MAX / 8)
+    return fail(TTS_ERR_INVALID_ARG, "filter_sample: rows (below 2^28), n >= 1 and ldl >= n");
   if (n > kFilterMaxN)
     return fail(TTS_ERR_UNSUPPORTED_SHAPE,
                 "filter_sample: n=" + std::to_string(n) + " exceeds 262144");
@@ -641,7 +641,7 @@ tts_status tts_filter_sample(tts_ctx* c, const void* logits, int logits_f16, int
     r.min_p = how->min_p;
   }
   r.out = out;
-  return counted(launch_filter_sample(r, S(stream)), "filter_sample");
+  return counted(launch_filter_sample(r, c->device, S(stream)), "filter_sample");
 }
 
 // ---------------------------------------------------------------- ragged chunks

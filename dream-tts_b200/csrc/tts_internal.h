@@ -338,7 +338,7 @@ struct FilterSampleRequest {
   const float* min_p = nullptr;
   int* out = nullptr;
 };
-cudaError_t launch_filter_sample(const FilterSampleRequest& r, cudaStream_t st);
+cudaError_t launch_filter_sample(const FilterSampleRequest& r, int device, cudaStream_t st);
 cudaError_t launch_cast_f32_f16(const float* x, __half* y, long n, cudaStream_t st);
 // Prefill as decode rows (map[r] = (lane, offset)): per-row block-table copies and positions;
 // then each lane's position advanced by its row count.
