@@ -29,10 +29,11 @@ typedef unsigned long long u64;
 constexpr int kFsThreads = 512;
 constexpr int kFsWarps = kFsThreads / 32;
 constexpr int kFsBins = 1024;
+constexpr int kFsLoads = 8;      // 16-byte loads a thread has on their way
 constexpr int kFsCap = 1024;     // ids the first CTA sorts at once
+constexpr int kFsFew = 96;       // ... without looking closer first
 constexpr int kFsMaxCluster = 8;
 constexpr float kFsOctaves = 45.f;  // below 2^-45 a weight is 0
-constexpr double kFsPerOctave = (kFsBins - 1) / double(kFsOctaves);
 constexpr int kFsTwo = 19456;    // ids in a CTA's part up to which two CTAs share an SM
 constexpr double kFsOne = 17592186044416.0;  // 2^44: the weight of the row's maximum
 
@@ -45,8 +46,8 @@ struct FsSums {
     lo[i] = uint32_t(w), hi[i] = uint32_t(w >> 32), count[i] = c;
   }
   // One id more: the carry of the lower word goes up.
-  __device__ __forceinline__ void add(int i, u64 w) {
-    atomicAdd(&count[i], 1u);
+  __device__ __forceinline__ void add(int i, u64 w, bool with_count) {
+    if (with_count) atomicAdd(&count[i], 1u);
     if (!w) return;
     const uint32_t low = uint32_t(w), old = atomicAdd(&lo[i], low);
     const uint32_t up = uint32_t(w >> 32) + (old + low < old ? 1u : 0u);
@@ -57,21 +58,23 @@ struct FsSums {
 struct FsSmem {
   FsSums<kFsBins> bin;          // by bin, then running
   FsSums<256> digit;            // by 8 bits of the keys, in a bin too full to sort
-  u64 list[kFsCap];             // first CTA: gathered ids, key << 32 | ~id
-  u64 run[kFsCap];              // their running weights
+  alignas(16) u64 list[kFsCap];  // first CTA: gathered ids, key << 32 | ~id
+  u64 run[kFsCap];              // their running weights (before: this CTA's gathered ids)
   double exp_table[256];        // 2^(i / 256)
   u64 part[kFsWarps];
-  u64 best[kFsMaxCluster];      // by CTA: its maximum, key << 32 | ~id; later its share of a sum
+  float low[kFsWarps];
+  uint32_t floor[kFsMaxCluster];  // by CTA: its smallest value's bits
+  u64 share[2][kFsMaxCluster];  // one value of each CTA, two uses in turn
   u64 answer;                   // what one thread, or the first CTA, found
-  uint32_t filled;              // first CTA: ids gathered
-  uint32_t keys[1];             // this CTA's part of the row
+  uint32_t mine;                // ids this CTA gathers
+  int digit_at;                 // the part of the keys that a target falls into
+  u64 digit_below[2];           // and the weight and count above it
+  alignas(16) float x[4];       // this CTA's part of the row (a.per entries), -inf: not to be picked
 };
 
-TTS_DEV uint32_t fs_key(float f) {  // 0: the id cannot be picked
-  f += 0.f;                         // -0 counts as 0
-  return f > -INFINITY ? float_order_key(f) : 0u;
-}
-TTS_DEV float fs_value(uint32_t key) {
+// NaN is not to be picked, -0 is 0.
+TTS_DEV float fs_clean(float f) { return f > -INFINITY ? f + 0.f : -INFINITY; }
+TTS_DEV float fs_value(uint32_t key) {  // of float_order_key
   return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
@@ -81,24 +84,11 @@ TTS_DEV uint32_t ld_cluster(const uint32_t* p, uint32_t cta) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr(p, cta)) : "memory");
   return v;
 }
-TTS_DEV u64 ld_cluster(const u64* p, uint32_t cta) {
-  u64 v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(cluster_addr(p, cta)) : "memory");
-  return v;
-}
 TTS_DEV void st_cluster(uint32_t* p, uint32_t cta, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr(p, cta)), "r"(v) : "memory");
 }
 TTS_DEV void st_cluster(u64* p, uint32_t cta, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_addr(p, cta)), "l"(v) : "memory");
-}
-TTS_DEV uint32_t add_cluster(uint32_t* p, uint32_t cta, uint32_t v) {
-  uint32_t old;
-  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;"
-               : "=r"(old)
-               : "r"(cluster_addr(p, cta)), "r"(v)
-               : "memory");
-  return old;
 }
 TTS_DEV uint32_t cluster_size() {
   uint32_t r;
@@ -113,15 +103,15 @@ struct FsScale {
   float mx, per_bin;  // the row's maximum; bins per unit of x
   double c;           // log2(e) / T
   const double* table;
-  uint32_t top;       // the maximum's key
-  TTS_DEV int bin(uint32_t key) const {  // grows as the key falls
-    if (key == top) return 0;            // also where the maximum is infinite
-    return min(kFsBins - 1, int((mx - fs_value(key)) * per_bin));
+  // Grows as x falls (0 for the maximum, also where the scale is infinite and this is 0 times it).
+  TTS_DEV int bin(float x) const { return min(kFsBins - 1, int((mx - x) * per_bin)); }
+  // Values below and above all of the given bins', one bin wider than they are.
+  TTS_DEV void bounds(int bin0, int bin1, float* low, float* high) const {
+    *low = bin1 == kFsBins - 1 ? -INFINITY : mx - (bin1 + 2) / per_bin;
+    *high = bin0 < 2 ? INFINITY : mx - (bin0 - 1) / per_bin;
   }
-  TTS_DEV u64 weight(uint32_t key) const {
-    if (key == top) return u64(1) << 44;
-    const double t = (double(fs_value(key)) - double(mx)) * c;
-    if (!(t > -double(kFsOctaves))) return 0;
+  TTS_DEV u64 weight(float x) const {
+    const double t = (double(x) - double(mx)) * c;
     const double magic = 26388279066624.;  // 1.5 * 2^44: one unit of the sum's last place is 2^-8
     const double s = t + magic;
     const int i = __double2loint(s);
@@ -134,7 +124,8 @@ struct FsScale {
     // times 2^(44 + i / 256) by the exponent, then rounded to an integer by the last place of 2^52
     const double f = __hiloint2double(__double2hiint(v) + ((44 + (i >> 8)) << 20),
                                       __double2loint(v));
-    return u64(__double_as_longlong(f + 4503599627370496.)) & 0xfffffffffffffull;
+    const u64 w = u64(__double_as_longlong(f + 4503599627370496.)) & 0xfffffffffffffull;
+    return t > -double(kFsOctaves) ? w : 0;  // no branch: the steps above are harmless for any t
   }
 };
 
@@ -162,7 +153,8 @@ TTS_DEV u64 fs_before(FsSmem& S, u64 v) {
   if ((threadIdx.x & 31) == 31) S.part[threadIdx.x >> 5] = inc;
   __syncthreads();
   u64 r = inc - v;
-  for (int i = 0; i < int(threadIdx.x >> 5); ++i) r += S.part[i];
+#pragma unroll
+  for (int i = 0; i < kFsWarps - 1; ++i) r += i < int(threadIdx.x >> 5) ? S.part[i] : 0;
   return r;
 }
 
@@ -180,70 +172,130 @@ TTS_DEV void fs_join(FsSums<N>& s, uint32_t rank, uint32_t ctas) {
   cluster_sync();
   if (ctas == 1) return;
   const int share = (N + int(ctas) - 1) / int(ctas), b0 = int(rank) * share;
-  for (int b = b0 + int(threadIdx.x); b < min(N, b0 + share); b += kFsThreads) {
+  for (int e = threadIdx.x; e < 2 * share; e += kFsThreads) {
+    const int b = b0 + (e >> 1);  // an entry's count and its weight by a thread each
+    if (b >= N) continue;
+    uint32_t l[kFsMaxCluster], h[kFsMaxCluster];
+#pragma unroll
+    for (uint32_t i = 0; i < kFsMaxCluster; ++i) {
+      l[i] = i < ctas ? ld_cluster(e & 1 ? &s.lo[b] : &s.count[b], i) : 0;
+      h[i] = i < ctas && (e & 1) ? ld_cluster(&s.hi[b], i) : 0;
+    }
     u64 w = 0;
-    uint32_t c = 0;
-    for (uint32_t i = 0; i < ctas; ++i) {
-      w += (u64(ld_cluster(&s.hi[b], i)) << 32) + ld_cluster(&s.lo[b], i);
-      c += ld_cluster(&s.count[b], i);
-    }
-    for (uint32_t i = 0; i < ctas; ++i) {  // only this CTA reads or writes these entries
-      st_cluster(&s.lo[b], i, uint32_t(w));
-      st_cluster(&s.hi[b], i, uint32_t(w >> 32));
-      st_cluster(&s.count[b], i, c);
+#pragma unroll
+    for (uint32_t i = 0; i < kFsMaxCluster; ++i) w += (u64(h[i]) << 32) + l[i];
+    for (uint32_t i = 0; i < ctas; ++i) {  // only this thread reads or writes these words
+      st_cluster(e & 1 ? &s.lo[b] : &s.count[b], i, uint32_t(w));
+      if (e & 1) st_cluster(&s.hi[b], i, uint32_t(w >> 32));
     }
   }
   cluster_sync();
 }
 
-// The sum of v over the row's CTAs (v alike in a CTA's threads).
-TTS_DEV u64 fs_sum_row(FsSmem& S, u64 v, uint32_t rank, uint32_t ctas) {
-  if (ctas == 1) return v;
-  cluster_sync();  // the last use of `best`
-  if (threadIdx.x < ctas) st_cluster(&S.best[rank], threadIdx.x, v);
-  cluster_sync();
-  u64 r = 0;
-  for (uint32_t i = 0; i < ctas; ++i) r += S.best[i];
-  return r;
+// Every CTA's v (alike in its threads) in all of the row's CTAs. One cluster barrier: the array is
+// used two uses later at the earliest, when all have passed the next use's barrier and so have
+// read this one.
+struct FsShare {
+  int turn = 0;
+  TTS_DEV const u64* operator()(FsSmem& S, u64 v, uint32_t rank, uint32_t ctas) {
+    u64* at = S.share[turn];
+    turn ^= 1;
+    if (threadIdx.x < ctas) st_cluster(&at[rank], threadIdx.x, v);
+    cluster_sync();
+    return at;
+  }
+};
+
+// f(i, x) for this CTA's `n` values that may be picked, four to a load.
+template <typename F>
+TTS_DEV void fs_each(const FsSmem& S, int n, F f) {
+  for (int i = threadIdx.x * 4; i < n; i += kFsThreads * 4) {
+    const float4 v = *reinterpret_cast<const float4*>(S.x + i);  // padded to fours with -inf
+    if (v.x > -INFINITY) f(i, v.x);
+    if (v.y > -INFINITY) f(i + 1, v.y);
+    if (v.z > -INFINITY) f(i + 2, v.z);
+    if (v.w > -INFINITY) f(i + 3, v.w);
+  }
 }
 
-// Puts this CTA's ids of the given bins and keys into the first CTA's list.
-TTS_DEV void fs_gather(FsSmem& S, const FsScale& r, int n, int id0, int bin0, int bin1,
-                       uint32_t key0, uint32_t key1) {
-  for (int i = threadIdx.x; i < n; i += kFsThreads) {
-    const uint32_t k = S.keys[i];
-    if (k < key0 || k > key1 || k == 0) continue;
-    const int b = r.bin(k);
-    if (b < bin0 || b > bin1) continue;
-    const uint32_t at = add_cluster(&S.filled, 0, 1u);
-    if (at < uint32_t(kFsCap)) st_cluster(&S.list[at], 0, (u64(k) << 32) | uint32_t(~(id0 + i)));
-  }
-  cluster_sync();
-}
-// First CTA: sorts the list by key, then id, and runs its weights up. Returns its length.
-TTS_DEV int fs_sort(FsSmem& S, const FsScale& r) {
-  const int t = threadIdx.x, m = min(int(S.filled), kFsCap);
-  int size = 32;
-  while (size < m) size *= 2;
+// Counts the row's ids of the given bins and keys and, if the first CTA's list holds them all, puts
+// them there, each CTA's behind those of the CTAs before it.
+TTS_DEV int fs_gather(FsSmem& S, const FsScale& r, int n, int id0, uint32_t rank, uint32_t ctas,
+                      FsShare& share, int bin0, int bin1, uint32_t key0, uint32_t key1) {
+  const int t = threadIdx.x;
+  float low, high;
+  r.bounds(bin0, bin1, &low, &high);
   __syncthreads();
-  if (t == 0) S.filled = 0;
-  for (int i = m + t; i < size; i += kFsThreads) S.list[i] = 0;
-  for (int k = 2; k <= size; k *= 2)  // bitonic, larger first
-    for (int j = k / 2; j > 0; j /= 2) {
-      __syncthreads();
-      for (int e = t; e < size / 2; e += kFsThreads) {
-        const int i = (e / j) * 2 * j + e % j;
-        const u64 a = S.list[i], b = S.list[i + j];
-        if ((a < b) == ((i & k) == 0)) S.list[i] = b, S.list[i + j] = a;
-      }
+  if (t == 0) S.mine = 0;
+  __syncthreads();
+  fs_each(S, n, [&](int i, float x) {
+    if (x < low || x > high) return;
+    const int b = r.bin(x);
+    const uint32_t k = float_order_key(x);
+    if (b < bin0 || b > bin1 || k < key0 || k > key1) return;
+    const uint32_t at = atomicAdd(&S.mine, 1u);
+    if (at < uint32_t(kFsCap)) S.run[at] = (u64(k) << 32) | uint32_t(~(id0 + i));
+  });
+  __syncthreads();
+  const int m = int(S.mine);
+  const u64* of = share(S, u64(m), rank, ctas);
+  int all = 0, place = 0;
+  for (uint32_t i = 0; i < ctas; ++i) {
+    if (i == rank) place = all;
+    all += int(of[i]);
+  }
+  if (all <= kFsCap) {
+    for (int i = t; i < m; i += kFsThreads) st_cluster(&S.list[place + i], 0, S.run[i]);
+    cluster_sync();
+  }
+  return all;
+}
+// First CTA: sorts the list's m entries by key, then id, and runs their weights up.
+TTS_DEV void fs_sort(FsSmem& S, const FsScale& r, int m) {
+  const int t = threadIdx.x;
+  // Each entry's place is the number of larger ones: warps of 32 entries, and where those are few
+  // several warps to the same 32, each counting over a part of the list.
+  const int groups = (m + 31) / 32, parts = max(1, kFsWarps / groups);
+  const int each = (m + parts - 1) / parts;
+  const int pad = (m + 1) / 2 * 2;
+  if (t == 0 && pad > m) S.list[m] = 0;
+  int* place = reinterpret_cast<int*>(S.run);  // not in use now
+  for (int i = t; i < m; i += kFsThreads) place[i] = 0;
+  __syncthreads();
+  u64 e[2] = {0, 0};
+  int at[2] = {-1, -1};
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int wp = (t >> 5) + u * kFsWarps;
+    const int g = wp % groups, part = wp / groups;
+    if (part >= parts || (u == 1 && groups <= kFsWarps)) continue;
+    const int i = g * 32 + (t & 31);
+    if (part == 0 && i < m) e[u] = S.list[i], at[u] = i;
+    const u64 mine = i < m ? S.list[i] : ~0ull;
+    int larger = 0;
+    const int from = part * each & ~1, to = part == parts - 1 ? pad : min(pad, (part + 1) * each & ~1);
+#pragma unroll 4
+    for (int j = from; j < to; j += 2) {
+      const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&S.list[j]);
+      larger += (x.x > mine) + (x.y > mine);
     }
+    if (i < m && larger) atomicAdd(&place[i], larger);
+  }
+  __syncthreads();
+  int to[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) to[u] = at[u] >= 0 ? place[at[u]] : 0;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (at[u] >= 0) S.list[to[u]] = e[u];
   __syncthreads();
   constexpr int kPer = kFsCap / kFsThreads;
   u64 w[kPer], sum = 0;
 #pragma unroll
   for (int u = 0; u < kPer; ++u) {
     const int i = t * kPer + u;
-    w[u] = i < m ? r.weight(uint32_t(S.list[i] >> 32)) : 0;
+    w[u] = i < m ? r.weight(fs_value(uint32_t(S.list[i] >> 32))) : 0;
     sum += w[u];
   }
   sum = fs_before(S, sum);
@@ -253,76 +305,113 @@ TTS_DEV int fs_sort(FsSmem& S, const FsScale& r) {
     S.run[t * kPer + u] = sum;
   }
   __syncthreads();
-  return m;
+}
+
+// Which of the 256 parts the running count (`ids`) or weight reaches `rest` in, from the largest
+// keys down; `rest` and `below` move to that part's start. Returns the part.
+TTS_DEV int fs_part(FsSmem& S, bool ids, u64* rest, u64* below) {
+  const int t = threadIdx.x, part = 255 - t;
+  const u64 w = t < 256 ? S.digit.weight(part) : 0, c = t < 256 ? S.digit.count[part] : 0;
+  const u64 w0 = fs_before(S, w), c0 = fs_before(S, c);
+  const u64 step = ids ? c : w, step0 = ids ? c0 : w0;
+  if (t < 256 && step0 < *rest && *rest <= step0 + step) {
+    S.digit_at = part;
+    S.digit_below[0] = w0;
+    S.digit_below[1] = c0;
+  }
+  __syncthreads();
+  *below += S.digit_below[0];
+  *rest -= S.digit_below[ids ? 1 : 0];
+  return S.digit_at;
 }
 
 // Where the running count (`ids`) or weight of the order reaches `target` (at least 1, at most
 // all): the weight up to there, the id there included. With `out` that id goes there. All of the
 // row's CTAs call it.
 TTS_DEV u64 fs_resolve(FsSmem& S, const FsScale& r, int n, int id0, uint32_t rank, uint32_t ctas,
-                       bool ids, u64 target, int* out) {
+                       FsShare& share, bool ids, u64 target, int* out) {
   const int t = threadIdx.x;
   const int bin = fs_reach(S, kFsBins, target, [&](int i) {
     return ids ? u64(S.bin.count[i]) : S.bin.weight(i);
   });
   u64 below = bin ? S.bin.weight(bin - 1) : 0;  // the weight of the ids before those looked at
-  const uint32_t before = bin ? S.bin.count[bin - 1] : 0;
-  uint32_t members = S.bin.count[bin] - before;
-  u64 rest = target - (ids ? u64(before) : below);
+  u64 rest = target - (ids ? (bin ? u64(S.bin.count[bin - 1]) : 0) : below);
   uint32_t key0 = 1, key1 = 0xffffffffu;
-  for (int shift = 24; members > uint32_t(kFsCap) && shift >= 0; shift -= 8) {
+  int members = fs_gather(S, r, n, id0, rank, ctas, share, bin, bin, key0, key1);
+  {
+    float low, high;
+    r.bounds(bin, bin, &low, &high);
+    key0 = max(float_order_key(low), 1u), key1 = float_order_key(high);
+  }
+  while (members > kFsCap && key0 < key1) {
+    // 256 equal parts of the keys, then the one that the target falls into
+    const int shift = max(0, 24 - __clz(key1 - key0));
     __syncthreads();
     if (t < 256) S.digit.put(t, 0, 0);
     __syncthreads();
-    for (int i = t; i < n; i += kFsThreads) {
-      const uint32_t k = S.keys[i];
-      if (k < key0 || k > key1 || k == 0 || r.bin(k) != bin) continue;
-      S.digit.add((k >> shift) & 255, r.weight(k));
-    }
+    fs_each(S, n, [&](int, float x) {
+      const uint32_t k = float_order_key(x);
+      if (k >= key0 && k <= key1 && r.bin(x) == bin)
+        S.digit.add((k - key0) >> shift, r.weight(x), true);
+    });
     fs_join(S.digit, rank, ctas);
-    // every thread for itself: from the largest digit down
-    int d = 255;
-    for (; d > 0; --d) {
-      const u64 w = S.digit.weight(d), step = ids ? u64(S.digit.count[d]) : w;
-      if (step >= rest) break;
-      rest -= step;
-      below += w;
-    }
-    members = S.digit.count[d];
-    const uint32_t prefix = shift == 24 ? 0u : key0 & ~((256u << shift) - 1u);
-    key0 = prefix | (uint32_t(d) << shift);
-    key1 = key0 | ((1u << shift) - 1u);
+    const int d = fs_part(S, ids, &rest, &below);
+    members = int(S.digit.count[d]);
+    key0 += uint32_t(d) << shift;
+    key1 = key0 + min(key1 - key0, (1u << shift) - 1u);
     cluster_sync();  // all CTAs have read the sums
+    if (members <= kFsCap) fs_gather(S, r, n, id0, rank, ctas, share, bin, bin, key0, key1);
   }
-  if (members > uint32_t(kFsCap)) {
+  if (members > kFsCap) {
     // one key, too many ids: count along the ids
-    const u64 w = r.weight(key0), nth = ids ? rest : (rest + w - 1) / w;
+    const float x0 = fs_value(key0);
+    const u64 w = r.weight(x0), nth = ids ? rest : (rest + w - 1) / w;
     if (out) {
       u64 mine = 0;
-      for (int i = t; i < n; i += kFsThreads) mine += S.keys[i] == key0;
+      for (int i = t; i < n; i += kFsThreads) mine += S.x[i] == x0;
       mine = fs_sum(S, mine);
-      fs_sum_row(S, mine, rank, ctas);
+      const u64* of = share(S, mine, rank, ctas);
       u64 skip = nth - 1;  // ids with this key before the one wanted
-      if (ctas > 1)
-        for (uint32_t i = 0; i < rank; ++i) skip -= S.best[i];
+      for (uint32_t i = 0; i < rank; ++i) skip -= of[i];
       if (skip < mine) {  // (not where it fell below 0)
         // this CTA's: a thread a run of ids
         const int per = (n + kFsThreads - 1) / kFsThreads, lo = min(n, t * per),
                   hi = min(n, lo + per);
         u64 here = 0;
-        for (int i = lo; i < hi; ++i) here += S.keys[i] == key0;
+        for (int i = lo; i < hi; ++i) here += S.x[i] == x0;
         u64 k = skip - fs_before(S, here);
         for (int i = lo; i < hi && k < here; ++i)
-          if (S.keys[i] == key0 && k-- == 0) *out = id0 + i;
+          if (S.x[i] == x0 && k-- == 0) *out = id0 + i;
       }
     }
     return below + nth * w;
   }
-  fs_gather(S, r, n, id0, bin, bin, key0, key1);
   if (rank == 0) {
-    const int m = fs_sort(S, r);
-    const int at =
-        min(ids ? int(rest) - 1 : fs_reach(S, m, rest, [&](int i) { return S.run[i]; }), m - 1);
+    if (members > kFsFew && key0 < key1) {
+      // a list this long in parts first, and only the part that counts sorted
+      const int shift = max(0, 24 - __clz(key1 - key0));
+      if (t < 256) S.digit.put(t, 0, 0);
+      if (t == 0) S.mine = 0;
+      __syncthreads();
+      for (int i = t; i < members; i += kFsThreads) {
+        const uint32_t k = uint32_t(S.list[i] >> 32);
+        S.digit.add((k - key0) >> shift, r.weight(fs_value(k)), true);
+      }
+      __syncthreads();
+      const uint32_t d = uint32_t(fs_part(S, ids, &rest, &below));
+      for (int i = t; i < members; i += kFsThreads) {
+        const u64 e = S.list[i];
+        if ((uint32_t(e >> 32) - key0) >> shift == d) S.run[atomicAdd(&S.mine, 1u)] = e;
+      }
+      __syncthreads();
+      members = int(S.mine);
+      for (int i = t; i < members; i += kFsThreads) S.list[i] = S.run[i];
+      __syncthreads();
+    }
+    fs_sort(S, r, members);
+    const int at = min(
+        ids ? int(rest) - 1 : fs_reach(S, members, rest, [&](int i) { return S.run[i]; }),
+        members - 1);
     if (t < int(ctas)) st_cluster(&S.answer, t, below + S.run[at]);
     if (out && t == 0) *out = int(~uint32_t(S.list[at]));
   }
@@ -352,16 +441,40 @@ __global__ void __launch_bounds__(kFsThreads, 2) filter_sample_kernel(const FsAr
   int* out = a.r.out + row;
   for (int b = t; b < kFsBins; b += kFsThreads) S.bin.put(b, 0, 0);
   if (t < 256) S.exp_table[t] = exp2(t / 256.);
-  if (t == 0) S.filled = 0;
   // ---- the row's part, once, and its maximum with the first id that has it
   u64 best = 0;
-#pragma unroll 8
-  for (int i = t; i < n; i += kFsThreads) {
-    const uint32_t k = fs_key(float(x[i]));
-    S.keys[i] = k;
-    const u64 b = (u64(k) << 32) | uint32_t(~(id0 + i));
-    best = k && b > best ? b : best;
+  float top = -INFINITY, bottom = INFINITY;
+  int top_at = 0;
+  const auto take = [&](int i, float f) {
+    f = fs_clean(f);
+    S.x[i] = f;
+    if (f > top) top = f, top_at = i;
+    if (f > -INFINITY) bottom = fminf(bottom, f);
+  };
+  // 16-byte loads from the first aligned element on
+  constexpr int kVec = 16 / int(sizeof(T));
+  const int head =
+      min(n, int((16 - (reinterpret_cast<uintptr_t>(x) & 15)) % 16 / sizeof(T)));
+  const int body = (n - head) / kVec;
+  if (t < head) take(t, float(x[t]));
+  const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+  for (int i0 = t; i0 < body; i0 += kFsThreads * kFsLoads) {
+    uint4 v[kFsLoads];
+#pragma unroll
+    for (int u = 0; u < kFsLoads; ++u)
+      if (i0 + u * kFsThreads < body) v[u] = __ldcs(xv + i0 + u * kFsThreads);
+#pragma unroll
+    for (int u = 0; u < kFsLoads; ++u)
+      if (i0 + u * kFsThreads < body) {
+        const T* e = reinterpret_cast<const T*>(&v[u]);
+#pragma unroll
+        for (int w = 0; w < kVec; ++w)
+          take(head + (i0 + u * kFsThreads) * kVec + w, float(e[w]));
+      }
   }
+  for (int i = head + body * kVec + t; i < n; i += kFsThreads) take(i, float(x[i]));
+  if (t < 4 && n + t < (n + 3) / 4 * 4) S.x[n + t] = -INFINITY;
+  if (top > -INFINITY) best = (u64(float_order_key(top)) << 32) | uint32_t(~(id0 + top_at));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const u64 b = __shfl_xor_sync(0xffffffffu, best, o);
@@ -370,26 +483,51 @@ __global__ void __launch_bounds__(kFsThreads, 2) filter_sample_kernel(const FsAr
   if ((t & 31) == 0) S.part[t >> 5] = best;
   __syncthreads();
   for (int i = 0; i < kFsWarps; ++i) best = S.part[i] > best ? S.part[i] : best;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    bottom = fminf(bottom, __shfl_xor_sync(0xffffffffu, bottom, o));
+  if ((t & 31) == 0) S.low[t >> 5] = bottom;
+  __syncthreads();
+  for (int i = 0; i < kFsWarps; ++i) bottom = fminf(bottom, S.low[i]);
   cluster_sync();  // every CTA of the row has started
-  if (t < int(ctas)) st_cluster(&S.best[rank], t, best);
-  cluster_sync();
-  for (uint32_t i = 0; i < ctas; ++i) best = S.best[i] > best ? S.best[i] : best;
+  FsShare share;
+  {
+    if (t < int(ctas)) st_cluster(&S.floor[rank], t, __float_as_uint(bottom));
+    const u64* of = share(S, best, rank, ctas);
+    for (uint32_t i = 0; i < ctas; ++i) {
+      best = of[i] > best ? of[i] : best;
+      bottom = fminf(bottom, __uint_as_float(S.floor[i]));
+    }
+  }
   const float temp = a.r.temperature ? a.r.temperature[row] : 1.f;
   if (!best || !(temp > 0.f)) {  // no id can be picked, or the largest logit is
     if (rank == 0 && t == 0) *out = best ? int(~uint32_t(best)) : -1;
     return;
   }
   FsScale r;
-  r.top = uint32_t(best >> 32);
-  r.mx = fs_value(r.top);
+  r.mx = fs_value(uint32_t(best >> 32));
+  if (r.mx == INFINITY) {  // infinite logits share the draw
+    for (int i = t; i < n; i += kFsThreads) S.x[i] = S.x[i] == INFINITY ? 0.f : -INFINITY;
+    r.mx = bottom = 0.f;
+    __syncthreads();
+  }
   r.c = 1.4426950408889634 / double(temp);
-  r.per_bin = float(r.c * kFsPerOctave);
+  // the bins span what the row has, 45 octaves at most (weights behind them are 0)
+  const double octaves = (double(r.mx) - double(bottom)) * r.c;
+  r.per_bin = float(r.c * ((kFsBins - 1) / fmin(fmax(octaves, 1e-3), double(kFsOctaves))));
   r.table = S.exp_table;
   // ---- counts and weights by bin, of the whole row in each of its CTAs
-  for (int i = t; i < n; i += kFsThreads) {
-    const uint32_t k = S.keys[i];
-    if (!k) continue;
-    S.bin.add(r.bin(k), r.weight(k));
+  const int want = a.r.top_k ? a.r.top_k[row] : 0;
+  const bool counts = want > 0 && want < a.r.n;  // only top-k needs them
+  for (int i = t * 4; i < n; i += kFsThreads * 4) {
+    const float4 v = *reinterpret_cast<const float4*>(S.x + i);  // padded to fours with -inf
+    const float e[4] = {v.x, v.y, v.z, v.w};
+    u64 w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = r.weight(e[u]);  // side by side: a long chain each
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (e[u] > -INFINITY) S.bin.add(r.bin(e[u]), w[u], counts);
   }
   fs_join(S.bin, rank, ctas);
   {
@@ -413,9 +551,7 @@ __global__ void __launch_bounds__(kFsThreads, 2) filter_sample_kernel(const FsAr
   // ---- the cuts, then the draw (the same in all CTAs up to here and after each step)
   u64 left = S.bin.weight(kFsBins - 1);
   const u64 all = left;
-  const uint32_t have = S.bin.count[kFsBins - 1];
-  const int want = a.r.top_k ? a.r.top_k[row] : 0;
-  bool top_k = want > 0 && uint32_t(want) < have;
+  bool top_k = counts && uint32_t(want) < S.bin.count[kFsBins - 1];
   const float p = a.r.top_p ? a.r.top_p[row] : 1.f;
   const bool top_p = p < 1.f;
   const float mp = a.r.min_p ? a.r.min_p[row] : 0.f;
@@ -423,22 +559,21 @@ __global__ void __launch_bounds__(kFsThreads, 2) filter_sample_kernel(const FsAr
   const u64 least = mp > 0.f ? u64(ceil(fmin(double(mp), 1.) * kFsOne)) : 0;
   const float draw = a.r.draws[row];
   const double u = draw > 0.f ? double(draw) : 0.;
-  int last = kFsBins;  // the bin that the first cut falls into
+  int m = kFsCap + 1;
   if (top_k) {
-    last = fs_reach(S, kFsBins, u64(want), [&](int i) { return u64(S.bin.count[i]); });
+    const int last = fs_reach(S, kFsBins, u64(want), [&](int i) { return u64(S.bin.count[i]); });
     // ids of no weight change nothing
-    if ((last ? S.bin.weight(last - 1) : 0) == all) top_k = false, last = kFsBins;
+    top_k = (last ? S.bin.weight(last - 1) : 0) < all;
+    if (top_k && S.bin.count[last] <= uint32_t(kFsCap))
+      m = fs_gather(S, r, n, id0, rank, ctas, share, 0, last, 1, 0xffffffffu);
   }
-  if (!top_k && top_p)
-    last = fs_reach(S, kFsBins, fs_target(double(p), left), [&](int i) { return S.bin.weight(i); });
   const auto run = [&](int i) { return S.run[i]; };
-  if (last < kFsBins && S.bin.count[last] <= uint32_t(kFsCap)) {
-    // few ids left: the first CTA takes them all
-    fs_gather(S, r, n, id0, 0, last, 1, 0xffffffffu);
+  if (m <= kFsCap) {
+    // few ids left: the first CTA has them all
     if (rank > 0) return;
-    int m = fs_sort(S, r);
-    if (top_k) m = want;
-    left = top_k ? S.run[m - 1] : all;
+    fs_sort(S, r, m);
+    m = want;
+    left = S.run[m - 1];
     if (top_p) {
       m = fs_reach(S, m, fs_target(double(p), left), run) + 1;
       left = S.run[m - 1];
@@ -454,23 +589,24 @@ __global__ void __launch_bounds__(kFsThreads, 2) filter_sample_kernel(const FsAr
     if (t == 0) *out = int(~uint32_t(S.list[min(at, m - 1)]));
     return;
   }
-  if (top_k) left = fs_resolve(S, r, n, id0, rank, ctas, true, u64(want), nullptr);
+  if (top_k) left = fs_resolve(S, r, n, id0, rank, ctas, share, true, u64(want), nullptr);
   if (top_p)
-    left = fs_resolve(S, r, n, id0, rank, ctas, false, fs_target(double(p), left), nullptr);
+    left = fs_resolve(S, r, n, id0, rank, ctas, share, false, fs_target(double(p), left), nullptr);
   if (least) {
     // whole bins pass up to the one before the threshold's neighbour; the three around it by id
-    const int bin = min(kFsBins - 1, int(-log2f(fminf(mp, 1.f)) * float(kFsPerOctave)));
+    const int bin = min(kFsBins - 1, int(-log2f(fminf(mp, 1.f)) * float(double(r.per_bin) / r.c)));
     u64 pass = 0;
-    for (int i = t; i < n; i += kFsThreads) {
-      const uint32_t k = S.keys[i];
-      if (!k || abs(r.bin(k) - bin) > 1) continue;
-      const u64 w = r.weight(k);
+    fs_each(S, n, [&](int, float x) {
+      if (abs(r.bin(x) - bin) > 1) return;
+      const u64 w = r.weight(x);
       pass += w >= least ? w : 0;
-    }
-    pass = fs_sum_row(S, fs_sum(S, pass), rank, ctas) + (bin > 1 ? S.bin.weight(bin - 2) : 0);
+    });
+    const u64* of = share(S, fs_sum(S, pass), rank, ctas);
+    pass = bin > 1 ? S.bin.weight(bin - 2) : 0;
+    for (uint32_t i = 0; i < ctas; ++i) pass += of[i];
     left = pass < left ? pass : left;
   }
-  fs_resolve(S, r, n, id0, rank, ctas, false, fs_target(u, left), out);
+  fs_resolve(S, r, n, id0, rank, ctas, share, false, fs_target(u, left), out);
   cluster_sync();  // no CTA leaves while another may still write to it
 }
 
@@ -484,9 +620,9 @@ cudaError_t launch_as(const FilterSampleRequest& r, int device, cudaStream_t st)
          ((r.n + ctas - 1) / ctas > kFsTwo ||
           (long(r.rows) * ctas * 2 <= 2 * sms && (r.n + ctas - 1) / ctas >= 4096)))
     ctas *= 2;
-  FsArgs a{r, (r.n + ctas - 1) / ctas};
+  FsArgs a{r, ((r.n + ctas - 1) / ctas + 7) / 8 * 8};
   static_assert(2 * (sizeof(FsSmem) + 4 * kFsTwo + 1024) <= 228 * 1024, "two CTAs an SM");
-  const size_t smem = sizeof(FsSmem) + sizeof(uint32_t) * a.per;
+  const size_t smem = sizeof(FsSmem) + sizeof(float) * a.per;
   {
     // the opt-in shared-memory limit is a per-device function attribute
     static std::mutex mu;
@@ -496,7 +632,7 @@ cudaError_t launch_as(const FilterSampleRequest& r, int device, cudaStream_t st)
       const cudaError_t e =
           cudaFuncSetAttribute(filter_sample_kernel<T>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               int(sizeof(FsSmem) + sizeof(uint32_t) * (kFilterMaxN / kFsMaxCluster)));
+                               int(sizeof(FsSmem) + sizeof(float) * (kFilterMaxN / kFsMaxCluster)));
       if (e != cudaSuccess) return e;
       done[device] = true;
     }
