@@ -33,7 +33,12 @@ def stream() -> C.c_void_p:
 
 def stream_of(t: torch.Tensor) -> int:
     """The current stream of the tensor's device (which need not be the current device)."""
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def as_type(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """t as contiguous `dtype` (a no-op `to` alone takes 2 us of a call's 10 on the host)."""
+    return (t if t.dtype == dtype else t.to(dtype)).contiguous()
 
 
 def ptr(t: torch.Tensor | None) -> C.c_void_p:

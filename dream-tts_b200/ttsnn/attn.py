@@ -42,6 +42,9 @@ def decode_attention_paged(q: torch.Tensor, kv: L.KvCache, spans: torch.Tensor, 
     return out
 
 
+_workspace: dict[int, int] = {}  # bytes of a chunk_attention call's workspace, by device
+
+
 def paged_cache(k: torch.Tensor, v: torch.Tensor, table: torch.Tensor) -> L.KvCache:
     """One layer's pools `[pages, n_kv, block_size, 128]` f16 and block table int32
     `[lanes, max_blocks]` as the cache the paged calls take (it keeps the tensors alive)."""
@@ -82,7 +85,9 @@ def chunk_attention(q: torch.Tensor, row_start: torch.Tensor, spans: torch.Tenso
     qc = q.contiguous()
     c = ctx_of(q)
     # from torch's allocator, so that calls on several streams or in several graphs have their own
-    size = int(L.load().tts_chunk_attention_workspace(c))
+    size = _workspace.get(q.device.index)
+    if size is None:
+        size = _workspace[q.device.index] = int(L.load().tts_chunk_attention_workspace(c))
     work = torch.empty(size, dtype=torch.uint8, device=q.device)
     L.call("tts_chunk_attention", c, qc.data_ptr(), int(q.dtype == torch.float16),
            heads // kv.n_kv, C.byref(b), C.byref(kv), float(scale), int(window), out.data_ptr(),

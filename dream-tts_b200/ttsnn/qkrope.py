@@ -6,7 +6,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from ._ctx import ctx_of, ptr, stream, stream_of
+from ._ctx import as_type, ctx_of, ptr, stream, stream_of
 
 
 def eligible(qkv: torch.Tensor, k_cache: torch.Tensor, head_dim: int) -> bool:
@@ -80,15 +80,16 @@ def chunk_batch(op: str, rows: int, row_start: torch.Tensor, spans: torch.Tensor
 
 
 def same_device(op: str, x: torch.Tensor, *others: torch.Tensor | None) -> None:
+    dev = x.device
     for t in others:
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{op}: tensors on {x.device} and {t.device}")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{op}: tensors on {dev} and {t.device}")
 
 
 def _tables(op: str, cos: torch.Tensor, sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if cos.shape != sin.shape or cos.dim() != 2:
         raise ValueError(f"{op}: cos and sin must be [positions, rotary_dim / 2] both")
-    return cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous()
+    return as_type(cos, torch.float32), as_type(sin, torch.float32)
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -151,9 +152,9 @@ def rotary_append(qkv: torch.Tensor, heads: int, row_start: torch.Tensor, spans:
     if rows == 0:
         return q
     x = qkv.contiguous()
-    nm = None if norms is None else norms.to(torch.float32).contiguous()
+    nm = None if norms is None else as_type(norms, torch.float32)
     L.call("tts_rotary_append", ctx_of(x), x.data_ptr(), int(x.dtype == torch.float16), int(heads),
-           C.byref(b), ptr(nm), float(eps), c.data_ptr(), s.data_ptr(), c.shape[0],
+           C.byref(b), None if nm is None else nm.data_ptr(), float(eps), c.data_ptr(), s.data_ptr(), c.shape[0],
            2 * c.shape[1], int(interleaved), C.byref(kv), q.data_ptr(),
            int(q.dtype == torch.float16), stream_of(x))
     return q

@@ -7,7 +7,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from ._ctx import ctx_of, ptr, stream, stream_of
+from ._ctx import as_type, ctx_of, ptr, stream, stream_of
 
 
 def argmax(logits: torch.Tensor, banned: torch.Tensor | None = None) -> torch.Tensor:
@@ -64,7 +64,7 @@ def _per_row(v, rows: int, dtype: torch.dtype, device: torch.device, name: str):
         return torch.full((rows,), v, dtype=dtype, device=device)
     if v.numel() != rows or v.device != device:
         raise ValueError(f"sample_filtered: {name} must hold one value per row, on {device}")
-    return v.to(dtype).contiguous()
+    return as_type(v, dtype)
 
 
 def sample_filtered(logits: torch.Tensor, draws: torch.Tensor, temperature=None, top_k=None,
