@@ -8,7 +8,9 @@
 //
 // A head is cut into slots of 8 dims that one thread loads, turns and stores, holding whole
 // pairs: in the half layout slot j < r/8 is dims 4j..4j+3 and r/2 + 4j..+3, else 8 consecutive
-// dims. The work is one read and one write of the rows; the table rows are shared by the heads.
+// dims. The work is one read and one write of the rows: bound by HBM. A thread keeps its slot
+// through several heads, so a row's table entries are read once for them, and has the heads' loads
+// on their way together.
 #include "chunk_batch.cuh"
 
 namespace tts {
@@ -31,12 +33,6 @@ struct Vec4<float> {
 };
 template <>
 struct Vec4<__half> {
-  static TTS_DEV void load(const __half* p, float* v) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-  }
   static TTS_DEV void store(__half* p, const float* v) {
     uint2 u;
     *reinterpret_cast<__half2*>(&u.x) = __floats2half2_rn(v[0], v[1]);
@@ -63,11 +59,57 @@ TTS_DEV Slot slot_of(int j, int rotary, int interleaved) {
   return s;
 }
 
+// A slot's 8 values as they are in memory (a thread has several heads' on their way) and as
+// numbers; f16 dims that are consecutive go 16 bytes at once.
+template <typename T>
+struct Raw {
+  uint32_t w[2 * sizeof(T)];
+  TTS_DEV void load(const T* head, const Slot& s) {
+    if (sizeof(T) == 4 || s.d1 == s.d0 + 4) {
+      const uint4 a = *reinterpret_cast<const uint4*>(head + s.d0);
+      w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+    }
+    if (sizeof(T) == 4) {
+      const uint4 b = *reinterpret_cast<const uint4*>(head + s.d1);
+      w[sizeof(T) * 2 - 4] = b.x, w[sizeof(T) * 2 - 3] = b.y;
+      w[sizeof(T) * 2 - 2] = b.z, w[sizeof(T) * 2 - 1] = b.w;
+    } else if (s.d1 != s.d0 + 4) {
+      const uint2 a = *reinterpret_cast<const uint2*>(head + s.d0);
+      const uint2 b = *reinterpret_cast<const uint2*>(head + s.d1);
+      w[0] = a.x, w[1] = a.y, w[2] = b.x, w[3] = b.y;
+    }
+  }
+  TTS_DEV void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (sizeof(T) == 4) {
+        v[i] = __uint_as_float(w[i % (2 * sizeof(T))]);
+      } else if (i % 2 == 0) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i / 2]));
+        v[i] = f.x, v[i + 1] = f.y;
+      }
+    }
+  }
+  static TTS_DEV void store(T* head, const Slot& s, const float* v) {
+    if (sizeof(T) == 2 && s.d1 == s.d0 + 4) {
+      uint4 u;
+      __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+      *reinterpret_cast<uint4*>(head + s.d0) = u;
+    } else {
+      Vec4<T>::store(head + s.d0, v);
+      Vec4<T>::store(head + s.d1, v + 4);
+    }
+  }
+};
+
 // Rotates the slot's 8 values by the 4 angles from table entry 4j.
-TTS_DEV void turn(float* v, const float* c, const float* s, int interleaved) {
+template <bool kInter>
+TTS_DEV void turn(float* v, const float* c, const float* s) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int ia = interleaved ? 2 * i : i, ib = interleaved ? 2 * i + 1 : i + 4;
+    const int ia = kInter ? 2 * i : i, ib = kInter ? 2 * i + 1 : i + 4;
     const float a = v[ia], b = v[ib];
     v[ia] = a * c[i] - b * s[i];
     v[ib] = b * c[i] + a * s[i];
@@ -85,65 +127,31 @@ struct RotaryArgs {
   int* err;
 };
 
-// A thread per (row, head, slot).
+// heads of one slot a thread takes at once: 128 bytes
 template <typename T>
-__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a) {
-  const int slots = a.hd / 8;
-  const long total = (long)a.rows * a.heads * slots;
-  for (long e = blockIdx.x * (long)kRotThreads + threadIdx.x; e < total;
-       e += (long)gridDim.x * kRotThreads) {
-    const int j = int(e % slots);
-    const long rh = e / slots;
-    const int h = int(rh % a.heads), row = int(rh / a.heads);
+constexpr int kRotHeads = 16 / int(sizeof(T));
+
+// A CTA takes `tile` rows; a thread a row's slot in kRotHeads heads, `per` = ceil(heads /
+// that) heads apart (neighbouring threads read neighbouring slots and heads).
+template <typename T, bool kInter>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a, int tile) {
+  constexpr int kHeads = kRotHeads<T>;
+  const int slots = a.hd / 8, per = (a.heads + kHeads - 1) / kHeads;
+  const int items = per * slots;
+  const int row0 = blockIdx.x * tile, rows = min(tile, a.rows - row0);
+  for (int e = threadIdx.x; e < rows * items; e += kRotThreads) {
+    const int row = row0 + e / items, in = e % items;
+    const int j = in % slots, h0 = in / slots;
+    const Slot s = slot_of(j, a.rotary, kInter);
+    const T* src = static_cast<const T*>(a.x) + (size_t)row * a.ldx + (size_t)h0 * a.hd;
+    T* dst = static_cast<T*>(a.y) + (size_t)row * a.ldy + (size_t)h0 * a.hd;
+    Raw<T> x[kHeads];
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u)
+      if (h0 + u * per < a.heads) x[u].load(src + (size_t)u * per * a.hd, s);
     const int pos = a.positions[row];
     if (pos < 0 || pos >= a.rope_len) {
-      if (h == 0 && j == 0) atomicOr(a.err, kFlagRopeRange);
-      continue;
-    }
-    const Slot s = slot_of(j, a.rotary, a.interleaved);
-    const T* src = static_cast<const T*>(a.x) + (size_t)row * a.ldx + (size_t)h * a.hd;
-    T* dst = static_cast<T*>(a.y) + (size_t)row * a.ldy + (size_t)h * a.hd;
-    float v[8];
-    Vec4<T>::load(src + s.d0, v);
-    Vec4<T>::load(src + s.d1, v + 4);
-    if (s.turned) {
-      float c[4], sn[4];
-      Vec4<float>::load(a.cos_t + (size_t)pos * (a.rotary / 2) + j * 4, c);
-      Vec4<float>::load(a.sin_t + (size_t)pos * (a.rotary / 2) + j * 4, sn);
-      turn(v, c, sn, a.interleaved);
-    }
-    Vec4<T>::store(dst + s.d0, v);
-    Vec4<T>::store(dst + s.d1, v + 4);
-  }
-}
-
-// One CTA per run of rows; half a warp per head of a row (16 slots of 8 dims), so the QK-norm's
-// sum of squares is four exchanges.
-template <typename TX, typename TQ>
-__global__ void __launch_bounds__(kRotThreads) rotary_append_kernel(const RotaryAppendRequest a) {
-  __shared__ int starts[kChunkMaxLanes + 1];
-  const int t = threadIdx.x;
-  for (int i = t; i <= a.lanes; i += kRotThreads) starts[i] = a.row_start[i];
-  __syncthreads();
-  if (!__syncthreads_and(chunk_starts_ok(starts, a.lanes, a.rows, t, kRotThreads))) {
-    if (t == 0 && blockIdx.x == 0) atomicOr(a.err, kFlagChunkStarts);
-    return;
-  }
-  const int j = t & 15, group = t >> 4;
-  const int all = a.heads + 2 * a.n_kv;
-  const Slot s = slot_of(j, a.rotary, a.interleaved);
-  const long cap = (long)a.max_blocks * a.block_size;
-  for (int row = starts[0] + blockIdx.x; row < starts[a.lanes]; row += gridDim.x) {
-    const int lane = chunk_lane_of(starts, a.lanes, row);
-    const int span = a.spans[lane];
-    const int pos = span - (starts[lane + 1] - row);
-    if (span > cap || pos < 0 || pos >= a.rope_len) {
-      if (t == 0) atomicOr(a.err, kFlagRopeRange);
-      continue;
-    }
-    const int page = a.block_table[(size_t)lane * a.max_blocks + pos / a.block_size];
-    if (page < 0 || page >= a.num_blocks) {
-      if (t == 0) atomicOr(a.err, kFlagPageRange);
+      if (in == 0) atomicOr(a.err, kFlagRopeRange);
       continue;
     }
     float c[4], sn[4];
@@ -151,53 +159,119 @@ __global__ void __launch_bounds__(kRotThreads) rotary_append_kernel(const Rotary
       Vec4<float>::load(a.cos_t + (size_t)pos * (a.rotary / 2) + j * 4, c);
       Vec4<float>::load(a.sin_t + (size_t)pos * (a.rotary / 2) + j * 4, sn);
     }
-    const size_t slot = (size_t)page * a.n_kv * a.block_size + pos % a.block_size;
-    for (int h0 = 0; h0 < all; h0 += kRotThreads / 16) {
-      const int h = h0 + group;
-      const bool live = h < all;
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      if (h0 + u * per >= a.heads) break;
       float v[8];
-      if (live) {
-        const TX* src = static_cast<const TX*>(a.x) + ((size_t)row * all + h) * 128;
-        Vec4<TX>::load(src + s.d0, v);
-        Vec4<TX>::load(src + s.d1, v + 4);
-      }
-      const bool qk = live && h < a.heads + a.n_kv;
-      if (a.norms) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += qk ? v[i] * v[i] : 0.f;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (qk) {
-          const float r = 1.f / sqrtf(ss * (1.f / 128.f) + a.eps);
-          const float* w = a.norms + (h < a.heads ? 0 : 128);
-          float w8[8];
-          Vec4<float>::load(w + s.d0, w8);
-          Vec4<float>::load(w + s.d1, w8 + 4);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w8[i];
-        }
-      }
-      if (!live) continue;
-      if (qk && s.turned) turn(v, c, sn, a.interleaved);
-      if (h < a.heads) {
-        TQ* dst = static_cast<TQ*>(a.q_out) + ((size_t)row * a.heads + h) * 128;
-        Vec4<TQ>::store(dst + s.d0, v);
-        Vec4<TQ>::store(dst + s.d1, v + 4);
-      } else {
-        const int hk = h - a.heads;
-        __half* pool = hk < a.n_kv ? a.k_pool : a.v_pool;
-        __half* dst = pool + (slot + (size_t)(hk % a.n_kv) * a.block_size) * 128;
-        Vec4<__half>::store(dst + s.d0, v);
-        Vec4<__half>::store(dst + s.d1, v + 4);
-      }
+      x[u].get(v);
+      if (s.turned) turn<kInter>(v, c, sn);
+      Raw<T>::store(dst + (size_t)u * per * a.hd, s, v);
     }
   }
 }
 
-int grid_for(long items, long per) {
-  const long g = (items + per - 1) / per;
-  return int(g < 1 ? 1 : g > 148L * 32 ? 148L * 32 : g);
+// `wpr` warps a row (1, 2, 4 or 8: more where rows are few), half a warp a head (16 slots of 8
+// dims, so the QK-norm's sum of squares is four exchanges), kRotHeads of them at once; warps take
+// pairs of heads in turn.
+template <typename TX, typename TQ, bool kInter>
+__global__ void __launch_bounds__(kRotThreads, 3) rotary_append_kernel(const RotaryAppendRequest a,
+                                                                    int wpr) {
+  __shared__ int starts[kChunkMaxLanes + 1];
+  __shared__ alignas(16) float norms[256];
+  const int t = threadIdx.x;
+  if (a.norms) norms[t] = a.norms[t];
+  for (int i = t; i <= a.lanes; i += kRotThreads) starts[i] = a.row_start[i];
+  __syncthreads();
+  if (!__syncthreads_and(chunk_starts_ok(starts, a.lanes, a.rows, t, kRotThreads))) {
+    if (t == 0 && blockIdx.x == 0) atomicOr(a.err, kFlagChunkStarts);
+    return;
+  }
+  const int wl = t & 31, j = wl & 15, half = wl >> 4;
+  const int rows_at_once = kRotThreads / 32 / wpr, w = (t >> 5) % wpr;
+  const int all = a.heads + 2 * a.n_kv;
+  const Slot s = slot_of(j, a.rotary, kInter);
+  const long cap = (long)a.max_blocks * a.block_size;
+  constexpr int kHeads = kRotHeads<TX>;
+  for (int row = starts[0] + blockIdx.x * rows_at_once + (t >> 5) / wpr; row < starts[a.lanes];
+       row += gridDim.x * rows_at_once) {
+    const TX* src = static_cast<const TX*>(a.x) + (size_t)row * all * 128;
+    Raw<TX> x[kHeads];
+    const auto load = [&](int h0) {
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        const int h = h0 + 2 * wpr * u;
+        if (h < all) x[u].load(src + (size_t)h * 128, s);
+      }
+    };
+    int h0 = 2 * w + half;
+    load(h0);  // on their way while the row's place is looked up
+    const int lane = chunk_lane_of(starts, a.lanes, row);
+    const int span = a.spans[lane];
+    const int pos = span - (starts[lane + 1] - row);
+    if (span > cap || pos < 0 || pos >= a.rope_len) {
+      if (wl == 0) atomicOr(a.err, kFlagRopeRange);
+      continue;
+    }
+    float c[4], sn[4];
+    if (s.turned) {
+      Vec4<float>::load(a.cos_t + (size_t)pos * (a.rotary / 2) + j * 4, c);
+      Vec4<float>::load(a.sin_t + (size_t)pos * (a.rotary / 2) + j * 4, sn);
+    }
+    const int page = a.block_table[(size_t)lane * a.max_blocks + pos / a.block_size];
+    if (page < 0 || page >= a.num_blocks) {
+      if (wl == 0) atomicOr(a.err, kFlagPageRange);
+      continue;
+    }
+    const size_t slot = (size_t)page * a.n_kv * a.block_size + pos % a.block_size;
+    for (;;) {
+#pragma unroll
+      for (int u = 0; u < kHeads; ++u) {
+        const int h = h0 + 2 * wpr * u;
+        const bool q = h < a.heads, k = !q && h < a.heads + a.n_kv;
+        float v[8];
+        x[u].get(v);
+        if (a.norms) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss += q || k ? v[i] * v[i] : 0.f;
+#pragma unroll
+          for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          if (q || k) {
+            const float r = 1.f / sqrtf(ss * (1.f / 128.f) + a.eps);
+            float n[8];
+            Vec4<float>::load(&norms[q ? 0 : 128] + s.d0, n);
+            Vec4<float>::load(&norms[q ? 0 : 128] + s.d1, n + 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * r * n[i];
+          }
+        }
+        if (h >= all) continue;
+        if ((q || k) && s.turned) turn<kInter>(v, c, sn);
+        if (q) {
+          Raw<TQ>::store(static_cast<TQ*>(a.q_out) + ((size_t)row * a.heads + h) * 128, s, v);
+        } else {
+          const int hk = h - a.heads - (k ? 0 : a.n_kv);
+          Raw<__half>::store((k ? a.k_pool : a.v_pool) + (slot + (size_t)hk * a.block_size) * 128,
+                             s, v);
+        }
+      }
+      h0 += 2 * wpr * kHeads;
+      if (h0 - half >= all) break;  // the same for the whole warp
+      load(h0);
+    }
+  }
+}
+
+template <bool kInter>
+void launch_append(const RotaryAppendRequest& r, int grid, int wpr, cudaStream_t st) {
+  if (r.x_f16 && r.q_f16)
+    rotary_append_kernel<__half, __half, kInter><<<grid, kRotThreads, 0, st>>>(r, wpr);
+  else if (r.x_f16)
+    rotary_append_kernel<__half, float, kInter><<<grid, kRotThreads, 0, st>>>(r, wpr);
+  else if (r.q_f16)
+    rotary_append_kernel<float, __half, kInter><<<grid, kRotThreads, 0, st>>>(r, wpr);
+  else
+    rotary_append_kernel<float, float, kInter><<<grid, kRotThreads, 0, st>>>(r, wpr);
 }
 
 }  // namespace
@@ -208,24 +282,34 @@ cudaError_t launch_rotary(const void* x, bool f16, int rows, int heads, int hd, 
                           cudaStream_t st) {
   RotaryArgs a{x,     y,     rows,     heads,  hd,          ldx, ldy, positions,
                cos_t, sin_t, rope_len, rotary, interleaved, err};
-  const int grid = grid_for((long)rows * heads * (hd / 8), kRotThreads);
-  if (f16)
-    rotary_kernel<__half><<<grid, kRotThreads, 0, st>>>(a);
+  // rows a CTA: enough to give each thread an item, at most 8
+  const int at_once = f16 ? kRotHeads<__half> : kRotHeads<float>;
+  const int items = (heads + at_once - 1) / at_once * (hd / 8);
+  int tile = 1;
+  while (tile < 8 && tile * items < kRotThreads) tile *= 2;
+  const int grid = (rows + tile - 1) / tile;
+  if (f16 && interleaved)
+    rotary_kernel<__half, true><<<grid, kRotThreads, 0, st>>>(a, tile);
+  else if (f16)
+    rotary_kernel<__half, false><<<grid, kRotThreads, 0, st>>>(a, tile);
+  else if (interleaved)
+    rotary_kernel<float, true><<<grid, kRotThreads, 0, st>>>(a, tile);
   else
-    rotary_kernel<float><<<grid, kRotThreads, 0, st>>>(a);
+    rotary_kernel<float, false><<<grid, kRotThreads, 0, st>>>(a, tile);
   return cudaGetLastError();
 }
 
-cudaError_t launch_rotary_append(const RotaryAppendRequest& r, cudaStream_t st) {
-  const int grid = grid_for(r.rows, 1);
-  if (r.x_f16 && r.q_f16)
-    rotary_append_kernel<__half, __half><<<grid, kRotThreads, 0, st>>>(r);
-  else if (r.x_f16)
-    rotary_append_kernel<__half, float><<<grid, kRotThreads, 0, st>>>(r);
-  else if (r.q_f16)
-    rotary_append_kernel<float, __half><<<grid, kRotThreads, 0, st>>>(r);
+cudaError_t launch_rotary_append(const RotaryAppendRequest& r, int device, cudaStream_t st) {
+  // as few warps a row as still fill the SMs (8 CTAs each)
+  const int sms = num_sms(device), full = sms * 8;
+  int wpr = 1;
+  while (wpr < 8 && (long)r.rows * wpr < (long)full * 8) wpr *= 2;
+  const int at_once = kRotThreads / 32 / wpr;
+  const int need = (r.rows + at_once - 1) / at_once, grid = need < full ? need : full;
+  if (r.interleaved)
+    launch_append<true>(r, grid, wpr, st);
   else
-    rotary_append_kernel<float, float><<<grid, kRotThreads, 0, st>>>(r);
+    launch_append<false>(r, grid, wpr, st);
   return cudaGetLastError();
 }
 

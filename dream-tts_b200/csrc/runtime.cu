@@ -745,7 +745,7 @@ tts_status tts_rotary_append(tts_ctx* c, const void* qkv, int qkv_f16, int heads
   r.v_pool = static_cast<__half*>(kv->v_pages);
   r.q_out = q_out;
   r.err = c->gemm.err;
-  return counted(launch_rotary_append(r, S(stream)), "rotary_append");
+  return counted(launch_rotary_append(r, c->device, S(stream)), "rotary_append");
 }
 
 tts_status tts_chunk_attention(tts_ctx* c, const void* q, int q_f16, int gqa,

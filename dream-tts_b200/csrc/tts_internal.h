@@ -304,7 +304,7 @@ struct RotaryAppendRequest {
   void* q_out = nullptr;  // [rows][heads][128]
   int* err = nullptr;
 };
-cudaError_t launch_rotary_append(const RotaryAppendRequest& r, cudaStream_t st);
+cudaError_t launch_rotary_append(const RotaryAppendRequest& r, int device, cudaStream_t st);
 // Attention of a ragged chunk over its lanes' pages (chunk_attn.cu).
 struct ChunkAttnRequest {
   const void* q = nullptr;  // [rows][n_kv * gqa][128]
