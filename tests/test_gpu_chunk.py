@@ -105,6 +105,68 @@ def test_chunk_attention_never_reads_unseen_positions(tt, window):
                 assert not np.isfinite(got[starts[i + 1] - 2:starts[i + 1]]).any()
 
 
+@pytest.mark.parametrize("rise", [1.0, -1.0, 0.0])
+@pytest.mark.parametrize("new,gqa", [(3, 1), (70, 4)])
+def test_chunk_attention_rising_scores(tt, rise, new, gqa):
+    """Scores that climb by hundreds of nats along the positions (the softmax's reference has to
+    follow inside a unit and from unit to unit), fall as steeply, or jump at a few places."""
+    b = ck.batch(31, [new], [900 - new], 1, 32)
+    starts, spans, table, k, v = b
+    at = np.arange(900)
+    size = (at / 3 if rise > 0 else (900 - at) / 3) if rise else np.where(at % 97 == 60, at / 5.0, 0)
+    row = np.zeros((900, 128))
+    row[:, 0] = size * SCALE ** -1 / 8
+    row[:, 1:] = np.random.default_rng(32).standard_normal((900, 127)) * 0.1
+    k[table[0, at // 32], 0, at % 32] = row.astype(np.float16)
+    q = np.random.default_rng(33).standard_normal((new, gqa, 128)).astype(np.float32)
+    q[..., 0] = 8
+    check_attention(tt, q.astype(np.float16), b)
+    check_attention(tt, q, b)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_chunk_attention_scales(tt, scale):
+    b = ck.batch(34, [33, 1], [200, 150], 2, 16)
+    starts, spans, table, k, v = b
+    q = np.random.default_rng(35).standard_normal((34, 4, 128)).astype(np.float16)
+    got = host(attend(tt, q, b, scale=scale))
+    want, mass = ck.attention(q, *b, scale, 0, np.zeros((34, 512)))
+    # f32 scores of up to ~100: their rounding (2^-24 each of 128 products and sums) adds to the bound
+    slack = 2.0 ** -24 * 128 * 40 * abs(scale) * mass
+    assert (np.abs(got - want) <= ck.attention_bound(want, mass) + slack).all()
+
+
+def test_chunk_attention_two_streams_at_once(tt):
+    """Calls that overlap on the GPU have a workspace each."""
+    args = []
+    for seed, (new, held) in ((36, ([1, 2], [5000, 4000])), (37, ([90, 260], [700, 0]))):
+        starts, spans, table, k, v = ck.batch(seed, new, held, 2, 32)
+        q = np.random.default_rng(seed).standard_normal((int(starts[-1]), 4, 128)).astype(np.float16)
+        kv = tt.attn.paged_cache(dev(k), dev(v), dev(table))
+        args.append((dev(q), dev(starts), dev(spans), kv, SCALE))
+    want = [tt.attn.chunk_attention(*a) for a in args]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for a, s in zip(args, streams):
+            with torch.cuda.stream(s):
+                got.append(tt.attn.chunk_attention(*a))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+    tt.check()
+
+
+def test_chunk_attention_many_lanes(tt):
+    """As many lanes as a call takes, most of them with one row or none."""
+    rng = np.random.default_rng(38)
+    new, held = rng.integers(0, 3, 1024), rng.integers(0, 40, 1024)
+    new[500], held[77] = 90, 700
+    b = ck.batch(39, new, held, 1, 8)
+    q = rng.standard_normal((int(b[0][-1]), 2, 128)).astype(np.float16)
+    check_attention(tt, q, b)
+
+
 def test_chunk_attention_pages_outside_pool(tt):
     b = ck.batch(11, [9, 40], [70, 30], 2, 16)
     starts, spans, table, k, v = b

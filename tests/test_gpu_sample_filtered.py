@@ -62,6 +62,35 @@ def test_equal_logits(tt):
          min_p=np.full(50, 0.5, np.float32))
 
 
+@pytest.mark.parametrize("n", [5003, 32003, 151851])
+def test_more_equal_logits_than_a_list_holds(tt, n):
+    """Thousands of ids share a logit (counted along the ids), a few values only, or lie so close
+    together beside one far off that their bin is narrowed by their bits, around zero too."""
+    rng = np.random.default_rng(n)
+    rows = 14
+    x = np.full((rows, n), -3.25, np.float32)
+    x[2:4] = np.round(rng.standard_normal((2, n)) * 2) / 2
+    x[4:6] = rng.integers(0, 2, (2, n)) * 0.5
+    x[6:10] = rng.standard_normal((4, n)) * 1e-3
+    x[8:10] += 7
+    x[6:10, n // 3] = 40
+    x[10:12] = rng.standard_normal((2, n)) * 1e-30
+    x[12:] = rng.standard_normal((2, n)) * 1e-3 - 100
+    x[12:, n - 1] = 1e8
+    u = rng.random(rows).astype(np.float32)
+    u[3], u[4] = 0, np.float32(1 - 2.0 ** -24)
+    t = np.full(rows, 20, np.float32)
+    t[12:] = 1e7
+    same(tt, x, u, temperature=t)
+    same(tt, x, u, temperature=t, top_k=rng.integers(1500, n, rows).astype(np.int32))
+    same(tt, x, u, temperature=t, top_p=rng.uniform(0.2, 0.999, rows).astype(np.float32))
+    same(tt, x, u, temperature=t, top_k=rng.integers(1500, n, rows).astype(np.int32),
+         top_p=rng.uniform(0.2, 0.999, rows).astype(np.float32), min_p=np.full(rows, 0.1, np.float32))
+    with np.errstate(over="ignore"):
+        half = x.astype(np.float16)
+    same(tt, half, u, top_p=np.full(rows, 0.7, np.float32))
+
+
 def test_settings_at_their_ends(tt):
     rng, x, u = inputs(10, 333, 3)
     nan = np.float32(np.nan)
