@@ -7,22 +7,33 @@
 // row f: token f / gqa, head f % gqa), so any group size shares one read of K and V. A work tile
 // is 256 flat rows as two 128-row query tiles (MMA M); its keys go by in units of 128 positions
 // (two MMAs a query tile and unit: S = Q.K^T, O += P.V). While one query tile's softmax runs, the
-// tensor cores work on the other.
+// tensor cores work on the other. Where there is one query tile only (a token or a few), its units
+// alternate between the two score buffers and groups of softmax warps, each with an O of its own,
+// and the first group reads both at the end (48 single rows over 4300 positions: 148 us; as two
+// query tiles, one of them empty, 182).
 //
 // Split. The units of all work tiles, one after another, are cut into equal runs, one per SM; a
 // work tile that a cut falls into leaves its parts (O, row maximum, row sum) in the workspace and
 // a second kernel joins them in order. So one long lane with one new token and a thousand short
 // chunks both use every SM, and results do not depend on timing.
 //
-// Warps 0-3 and 4-7: one query row a thread through softmax and output, query tiles 0 and 1.
-// Warps 8 and 11 load K and V (TMA boxes of whole 256-byte rows within a page), warp 9 issues the MMAs, warp 10 walks the work. S and then P (f16, in place)
-// stay in TMEM, O accumulates in TMEM.
+// Warps 0-3 and 4-7: one query row a thread through softmax and output, query tiles 0 and 1. Warps
+// 8 and 11 load K and V (TMA boxes of whole 256-byte rows within a page), warp 9 issues the MMAs,
+// warp 10 walks the work. P (f16) takes the place of S in TMEM and is the A operand of O += P.V.
 //
 // Softmax in powers of two against a reference r: w = 2^(c s - r + 8), c = scale log2 e. r is the
 // largest c s of the row's first unit and stays while the weights of 64 positions add up to no more
 // than f16 holds; only then O and the sum are brought to a new one (random scores hardly ever ask
 // for it after the first units), so no maximum is looked for in most units. Weights keep f16's 11
 // bits down to 2^-22 of r's; sums are f32.
+//
+// Measured (16 q heads, 8 kv heads): 4096 new rows over 12288 positions 439 us, 1096 TFLOP/s, 63 %
+// of the rate of a large plain product: a unit of two query tiles takes about 3.9k clocks, its MMAs
+// 2.4k to 2.9k and its exponentials 2.0k (16 a clock) of them, the rest is their hand-overs. 48
+// single rows over 4300 positions 148 us, 5.7 TB/s, 88 % of a copy: bound by HBM. 448 single rows
+// over 300: 197 us, 2.8 TB/s: a run of three units is too short to hide its start and end (210 us
+// with the queries loaded between runs, by the softmax warps; 325 with loops over a unit unrolled
+// and three copies of the loading code besides: instruction fetch).
 #include <mutex>
 
 #include "chunk_batch.cuh"
@@ -36,10 +47,13 @@ constexpr int kCaTile = 256;  // flat query rows of a work tile
 constexpr int kCaKeys = 128;  // positions of a unit
 constexpr int kCaSegs = 4;    // work descriptors in flight
 constexpr float kCaBias = 8.f, kCaMost = 65504.f;
-constexpr int kCaFirst = 64;  // positions of a unit whose weights the MMAs get first
+// The MMAs get the weights of half a unit while the other half's are on their way (4096 rows over
+// 12288 positions: in halves 436 us, 96 and 32 443, all 128 at once 518).
+constexpr int kCaHalf = kCaKeys / 2;
 
 // 128 rows x 128 f16 for the MMAs: groups of 8 rows, in each two halves of 64 columns, rows of 128
-// bytes with the 128-byte swizzle (what a TMA box of 64 columns x 8 rows x 2 halves x groups writes).
+// bytes with the 128-byte swizzle (what a TMA box of 64 columns x 8 rows x 2 halves x groups
+// writes).
 constexpr int kCaTileBytes = 128 * 256;
 TTS_DEV uint32_t ca_at(int r, int piece) {  // byte offset of 16-byte piece 0..15 of row r
   return uint32_t(r >> 3) * 2048u + uint32_t(piece >> 3) * 1024u + uint32_t(r & 7) * 128u +
@@ -107,8 +121,9 @@ template <int kK, int kV, int kParts>  // tiles of K and V in flight; f16 pieces
 struct CaSmem {
   uint8_t ring[kK + kV][kCaTileBytes];  // K's, then V's
   uint8_t q[2][kParts][kCaTileBytes];
-  uint64_t full[kK + kV], empty[kK + kV], q_full[2], s_full[2], h_full[2], h_done[2], p_full[2], o_full[2];
-  uint64_t seg_full[kCaSegs], seg_empty[kCaSegs], tail, drain, x_full, x_empty;
+  uint64_t full[kK + kV], empty[kK + kV];
+  uint64_t q_full[2], s_full[2], h_full[2], h_done[2], p_full[2], o_full[2];
+  uint64_t seg_full[kCaSegs], seg_empty[kCaSegs], seg_done[kCaSegs], tail, drain, x_full, x_empty;
   float x_ref[128], x_sum[128];  // the second group's, where one query tile has both groups
   CaSeg seg[kCaSegs];
   int start[4];  // the CTA's first lane, work tile, head and unit
@@ -122,11 +137,21 @@ struct Int {
   static constexpr int value = N;
 };
 
+// A run of no more rows than a warp loads at once: its queries are loaded by the warp that walks
+// the work, into the other buffer than the run before's if that was one too, while that is at work.
+// Any other run's are loaded by the softmax warps, tile tl's into buffer tl, when the run before is
+// done (a warp takes about a microsecond for 32 rows: chunks of 512 rows 149 us with all queries
+// loaded by the one, 106 this way).
+TTS_DEV bool ca_few(const CaSeg& s, int gqa) { return s.n * gqa - s.flat0 <= 32; }
+TTS_DEV int ca_q_buffer(bool few, bool last_few, int last) {
+  return few && last_few ? last ^ 1 : 0;
+}
+
 // A softmax thread's query row in a run.
 struct CaRow {
   int pr, f, pos, lo;  // in the work tile, flat in the lane; its position, the first it sees
   int rh;              // its row of q and out [rows * heads][128], -1: none
-  bool one, live, work;  // one query tile; a row at all; any in the warp
+  bool one, few, live, work;  // one query tile; ca_few; a row at all; any in the warp
 };
 
 // What a split work tile's part was, one per CTA for the run it takes over from the CTA before
@@ -143,7 +168,8 @@ struct CaArgs {
   int box;      // rows of a page that one copy takes
   int odd;      // one page per lane, of no multiple of 8 rows
   uint32_t div_m, div_s;  // p / block_size = p * div_m >> 32 + div_s for 0 <= p < 2^31
-  int wide;     // out is 32-byte aligned: whole sectors at a time
+  int wide;     // out is 32-byte aligned: whole sectors at a time (4600 rows of 16 heads, in chunks
+                // of up to 701: 138 us, in halves 144)
   CaPart* parts;
   float* part_data;
 };
@@ -222,6 +248,12 @@ TTS_DEV float ca_weights(const uint32_t* v, uint32_t* y, float c, float ref) {
   }
   const float2 s = add2(add2(part[0], part[1]), add2(part[2], part[3]));
   return s.x + s.y;
+}
+// Which of columns 0..31 lie in first .. last.
+TTS_DEV uint32_t ca_seen(int first, int last) {
+  const uint32_t from = first <= 0 ? 0xffffffffu : first > 31 ? 0u : 0xffffffffu << first;
+  const uint32_t to = last < 0 ? 0u : last >= 31 ? 0xffffffffu : (2u << last) - 1u;
+  return from & to;
 }
 // max(ref, c times the largest of N scores), NaN if a score is.
 template <int N>
@@ -495,6 +527,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     for (int i = 0; i < kCaSegs; ++i) {
       mbar_init(&S.seg_full[i], 1);
       mbar_init(&S.seg_empty[i], 11);
+      mbar_init(&S.seg_done[i], 1);  // all its scores are
     }
     mbar_init(&S.x_full, 4);
     mbar_init(&S.x_empty, 4);
@@ -533,7 +566,31 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     // ---- the work walk: units in order of lane, work tile, head
     int lane = S.start[0], k = S.start[1], head = S.start[2], off = S.start[3], left = S.count;
     CaLane l = ca_lane(r, lane);
-    for (;;) {
+    int buf = 0;
+    bool was_few = false;
+    // The queries of run i, if they are this warp's (the first run's never are). Their buffer is
+    // free once the scores of the run before are done, of the one before that if both are few. The
+    // wait cannot miss its phase: the slot's next run is not out yet, and all before are done.
+    const auto load_queries = [&](const CaSeg& s, int i) {
+      const bool few = ca_few(s, r.gqa);
+      const int free = i - (was_few ? 2 : 1);
+      buf = ca_q_buffer(few, was_few, buf);
+      was_few = few;
+      if (!few || i == 0) return;
+      if (free >= 0) ok = ca_wait(&S.seg_done[free % kCaSegs], (free / kCaSegs) & 1);
+      if (!ok) return;
+      const int f = s.flat0 + wl;
+      ca_load_q(S.q[buf], static_cast<const TQ*>(r.q),
+                f < s.n * r.gqa ? (s.row0 + f / r.gqa) * (r.n_kv * r.gqa) + s.head * r.gqa +
+                                      f % r.gqa
+                                : -1,
+                0, a.negate);  // (the tile's other rows' scores are not read)
+      fence_proxy_async();
+      __syncwarp();
+      if (wl < 4) mbar_arrive(&S.q_full[buf]);
+    };
+    CaSeg before{};
+    for (int i = 0;; ++i) {
       CaSeg s{};
       if (left > 0) {
         int first, count;
@@ -558,13 +615,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           p.valid = 1;
         }
       }
-      // its queries, which the softmax warps will want in a few microseconds, into L2
+      // its queries, wanted in a few microseconds, into L2
       const int lines = int(sizeof(TQ)) * r.gqa;  // of 128 bytes, per token and kv head
       const int q0 = s.flat0 / r.gqa, q1 = min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
-      for (int i = wl; i < (q1 - q0) * lines; i += 32)
+      for (int e = wl; e < (q1 - q0) * lines; e += 32)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(
             static_cast<const char*>(r.q) +
-            (((size_t)(s.row0 + q0 + i / lines) * r.n_kv + s.head) * lines + i % lines) * 128));
+            (((size_t)(s.row0 + q0 + e / lines) * r.n_kv + s.head) * lines + e % lines) * 128));
       ok = ca_wait(&S.seg_empty[seg_slot], seg_phase ^ 1);
       if (!ok) break;
       if (wl == 0) {
@@ -573,7 +630,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       }
       __syncwarp();
       if (++seg_slot == kCaSegs) seg_slot = 0, seg_phase ^= 1;
-      if (s.units == 0) break;
+      if (i > 0) load_queries(before, i - 1);
+      if (s.units == 0 || !ok) break;
+      before = s;
     }
   } else if (warp != 9) {
     // ---- warp 8 K, warp 11 V, by boxes of `box` rows of one page: warp lane g looks up box g, one
@@ -662,7 +721,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     // the P just read (MMAs of one thread run in the order of their issue).
     const uint32_t idesc_s = idesc_f16_f32(128, kCaKeys);
     const uint32_t idesc_o = idesc_f16_f32(128, 128) | (1u << 16);  // B (V) MN-major
-    int k_slot = 0, v_slot = 0;
+    int k_slot = 0, v_slot = 0, buf = 0, run = 0;
+    bool was_few = false;
     uint32_t k_phase = 0, v_phase = 0, q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
     const auto next_k = [&] {
       if (++k_slot == kK) k_slot = 0, k_phase ^= 1;
@@ -672,36 +732,44 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     const uint64_t q_desc = smem_desc(smem_u32(S.q), 16, 2048, 2);
     const uint64_t k_desc = smem_desc(smem_u32(S.ring), 16, 2048, 2);
     const uint64_t v_desc = smem_desc(smem_u32(S.ring[kK]), 1024, 2048, 2);
-    // S_buf = Q_tl.K^T
-    const auto scores = [&](int buf, int tl, int at) {
-      const uint64_t q = ca_desc(q_desc, tl * kParts * kTile16), k = ca_desc(k_desc, at * kTile16);
+    // S_tl = Q.K^T, Q from buffer `from`
+    const auto scores = [&](int tl, int from, int at, uint64_t* done) {
+      const uint64_t q = ca_desc(q_desc, from * kParts * kTile16);
+      const uint64_t k = ca_desc(k_desc, at * kTile16);
 #pragma unroll
       for (int h = 0; h < kParts; ++h)
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
           constexpr int kHalf16 = 1024 / 16;
           const int o = (kk >> 2) * kHalf16 + (kk & 3) * 2;
-          umma_f16(tmem + buf * 128, ca_desc(q, h * kTile16 + o), ca_desc(k, o), idesc_s,
+          umma_f16(tmem + tl * 128, ca_desc(q, h * kTile16 + o), ca_desc(k, o), idesc_s,
                    (h | kk) != 0);
         }
-      umma_commit(&S.s_full[buf]);
+      umma_commit(&S.s_full[tl]);
+      if (done) umma_commit(done);
     };
     CaSeg s;
     while (ok && (ok = next_seg(&s)) && s.units > 0) {
       // one query tile: units go to the two score buffers in turn, ahead of them the next but one
       const bool one = s.flat0 + 128 >= s.n * r.gqa;
       const int ahead = one ? 2 : 1;
+      const bool few = ca_few(s, r.gqa);
+      buf = ca_q_buffer(few, was_few, buf);
+      was_few = few;
+      uint64_t* const done = &S.seg_done[run++ % kCaSegs];  // after the run's last scores
       for (int b = 0; b < 2 && ok; ++b) {
         if (one && b >= s.units) break;
         if (b == 0 || one) ok = ca_wait(&S.full[k_slot], k_phase);
         if (ok && (b == 0 || !one)) {
-          ok = ca_wait(&S.q_full[b], q_phase[b]);
-          q_phase[b] ^= 1;
+          const int from = one ? buf : b;
+          ok = ca_wait(&S.q_full[from], q_phase[from]);
+          q_phase[from] ^= 1;
         }
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
-          scores(b, one ? 0 : b, k_slot);
+          const bool last = s.units == (one ? b + 1 : 1) && (one || b == 1);
+          scores(b, one ? buf : b, k_slot, last ? done : nullptr);
           if (one || b == 1) umma_commit(&S.empty[k_slot]);
         }
         __syncwarp();
@@ -721,7 +789,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kCaFirst / 16; ++kk) values(kk);
+            for (int kk = 0; kk < kCaHalf / 16; ++kk) values(kk);
             umma_commit(&S.h_done[b]);
           }
           __syncwarp();
@@ -732,9 +800,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int kk = kCaFirst / 16; kk < 8; ++kk) values(kk);
+            for (int kk = kCaHalf / 16; kk < 8; ++kk) values(kk);
             if (more)
-              scores(b, one ? 0 : b, k_slot);
+              scores(b, one ? buf : b, k_slot,
+                     j + ahead == s.units - 1 && (one || b == 1) ? done : nullptr);
             else
               umma_commit(&S.o_full[b]);
           }
@@ -768,6 +837,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       CaRow w;
       // one query tile only: its units alternate between the two groups of warps
       w.one = s.flat0 + 128 >= s.n * r.gqa;
+      w.few = ca_few(s, r.gqa);
       w.pr = (w.one ? 0 : tl * 128) + lane_row;
       w.f = s.flat0 + w.pr;
       w.live = w.f < s.n * r.gqa;
@@ -778,8 +848,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       w.rh = w.live ? (s.row0 + tok) * (r.n_kv * r.gqa) + s.head * r.gqa + w.f % r.gqa : -1;
       return w;
     };
-    const auto load_queries = [&](const CaSeg& s, const CaRow& w) {
-      if (s.units == 0 || (w.one && tl == 1)) return;
+    const auto load_queries = [&](const CaSeg& s, const CaRow& w, bool first) {
+      if (s.units == 0 || (w.one && tl == 1) || (w.few && !first)) return;
       ca_load_q(S.q[tl], static_cast<const TQ*>(r.q), w.rh, (warp & 3) * 32, a.negate);
       fence_proxy_async();
       tc_fence_before();
@@ -787,10 +857,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       if (wl == 0) mbar_arrive(&S.q_full[tl]);
     };
     CaSeg s{};
-    ok = next_seg(&s);
     CaRow w = rows_of(s);
-    if (ok) load_queries(s, w);
-    while (ok && s.units > 0) {
+    for (;;) {
       // rows of a warp see contiguous ranges: a unit inside all of them needs no mask
       const int pos_min = __reduce_min_sync(0xffffffffu, w.live ? w.pos : INT_MAX);
       const int lo_max = __reduce_max_sync(0xffffffffu, w.live ? w.lo : 0);
@@ -806,21 +874,24 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           const int p0 = (s.unit0 + j) * kCaKeys;
           const bool edge = p0 + kCaKeys - 1 > pos_min || p0 < lo_max;
           const int first = w.lo - p0, last = w.pos - p0;  // columns the row sees
-          uint32_t x[kCaKeys];
-          // a part of the unit's positions: their scores in x, their weights over them in TMEM
-          const auto step = [&](auto from, auto to) {
-            constexpr int c0 = decltype(from)::value, n = decltype(to)::value - c0;
+          // the unit's positions in two halves: their scores in x, their weights over them in TMEM
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t x[kCaHalf];
+            const int c0 = h * kCaHalf;
+            tmem_ld32(s_at + c0, x);
+            tmem_ld32(s_at + c0 + 32, x + 32);
             tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < n; e += 32) tmem_tie32(x + c0 + e);
-            if (c0 == 0) {
-#pragma unroll
-              for (int e = n; e < kCaKeys; e += 32) tmem_ld32(s_at + e, x + e);
-            }
+            tmem_tie32(x);
+            tmem_tie32(x + 32);
             if (edge) {
 #pragma unroll
-              for (int e = c0; e < c0 + n; ++e)
-                if (e < first || e > last) x[e] = 0xff800000u;  // -inf
+              for (int w32 = 0; w32 < 2; ++w32) {
+                const uint32_t seen = ca_seen(first - c0 - w32 * 32, last - c0 - w32 * 32);
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (!(seen >> e & 1u)) x[w32 * 32 + e] = 0xff800000u;  // -inf
+              }
             }
             float got = 0.f;
             bool raise = ref == -INFINITY, any = fresh;
@@ -830,19 +901,19 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 // O holds weights against the old reference: bring it, and the sum, to the new one
                 float up = ref;
                 if (raise) {
-                  up = ca_max<n>(x + c0, a.c, ref);
+                  up = ca_max<kCaHalf>(x, a.c, ref);
                   if (up == INFINITY) up = NAN;  // as the row's formula has it
                 }
                 const float keep = up == -INFINITY ? 1.f : ex2(ref - up);
                 ref = up;
                 sum *= keep;
                 fresh = __any_sync(0xffffffffu, ref == -INFINITY);
-                if (c0 > 0) {  // the first part's MMAs; before that, S(j) came after all others
+                if (h > 0) {  // the first half's MMAs; before that, S(j) came after all others
                   ok = ca_wait(&S.h_done[tl], s_phase ^ 1);
-                  if (!ok) return;
+                  if (!ok) break;
                   tc_fence_after();
                 }
-                if (j > step0 || c0 > 0) {
+                if (j > step0 || h > 0) {
 #pragma unroll 1
                   for (int i = 0; i < 8; ++i) {
                     float o[16];
@@ -854,25 +925,22 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                   }
                 }
               }
-              uint32_t y[n / 2];
-              got = ca_weights<n>(x + c0, y, a.c, ref);
-#pragma unroll
-              for (int e = 0; e < n / 2; e += 16) tmem_st16(s_at + c0 / 2 + e, y + e);
+              uint32_t y[kCaHalf / 2];
+              got = ca_weights<kCaHalf>(x, y, a.c, ref);
+              tmem_st16(s_at + c0 / 2, y);
+              tmem_st16(s_at + c0 / 2 + 16, y + 16);
               raise = !(got <= kCaMost) && ref == ref;
               any = __any_sync(0xffffffffu, raise);
               if (!any) break;
             }
+            if (!ok) break;
             sum += got;
             tmem_wait_st();
-          };
-#pragma unroll
-          for (int e = 0; e < kCaFirst; e += 32) tmem_ld32(s_at + e, x + e);
-          step(Int<0>(), Int<kCaFirst>());
-          if (ok) {  // the MMAs can start on the first part of P
-            tc_fence_before();
-            __syncwarp();
-            if (wl == 0) mbar_arrive(&S.h_full[tl]);
-            step(Int<kCaFirst>(), Int<kCaKeys>());
+            if (h == 0) {  // the MMAs can start on the first half of P
+              tc_fence_before();
+              __syncwarp();
+              if (wl == 0) mbar_arrive(&S.h_full[tl]);
+            }
           }
           if (!ok) break;
         } else if (wl == 0) {
@@ -883,75 +951,43 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         if (wl == 0) mbar_arrive(&S.p_full[tl]);
       }
       if (!ok) break;
-      // The next run's queries while the last MMAs are on their way: this tile's scores are all
-      // done. (Not where both groups work on one tile, the other's may not be.)
       CaSeg sn{};
       ok = next_seg(&sn);
       if (!ok) break;
       const CaRow wn = rows_of(sn);
-      if (!w.one) load_queries(sn, wn);
       if (step0 < s.units) {
         ok = ca_wait(&S.o_full[tl], o_phase);
         o_phase ^= 1;
         if (!ok) break;
         tc_fence_after();
       }
-      if (w.one && s.units > 1) {
-        // the second group hands over its reference, sum and O, 64 dims at a time, in the place
-        // of the second query tile
-        float* xo = reinterpret_cast<float*>(S.q[1][0]) + lane_row;
-        float mine = 1.f, other = 0.f;  // what the two groups' sums count
+      float mine = 1.f, other = 0.f;  // what the two groups' O and sums over one query tile count
+      if (w.one && s.units > 0) {
+        // the second group leaves its O, in the same TMEM lanes, to the first (and does not run
+        // ahead of it, to load a next run's queries over this one's)
         if (tl == 1) {
           S.x_ref[lane_row] = ref;
           S.x_sum[lane_row] = sum;
-        }
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          if (tl == 1) {
-#pragma unroll 1
-            for (int d = 0; d < 64 && w.work; d += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_at + h * 64 + d, o);
-              tmem_wait_ld();
-              tmem_tie32(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) xo[(d + e) * 128] = __uint_as_float(o[e]);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (wl == 0) mbar_arrive(&S.x_full);
-            ok = ca_wait(&S.x_empty, x_phase);
-          } else {
-            ok = ca_wait(&S.x_full, x_phase);
-            if (ok && h == 0) {
-              const float ref1 = S.x_ref[lane_row], top = max3(ref, ref1, ref1);
-              mine = ref == -INFINITY ? 0.f : ex2(ref - top);
-              other = ref1 == -INFINITY ? 0.f : ex2(ref1 - top);
-              sum = sum * mine + S.x_sum[lane_row] * other;
-              ref = top;
-            }
-#pragma unroll 1
-            for (int d = 0; d < 64 && w.work && ok; d += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_at + h * 64 + d, o);
-              tmem_wait_ld();
-              tmem_tie32(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                o[e] = __float_as_uint(fmaf(xo[(d + e) * 128], other, __uint_as_float(o[e]) * mine));
-              tmem_st16(o_at + h * 64 + d, o);
-              tmem_st16(o_at + h * 64 + d + 16, o + 16);
-              tmem_wait_st();
-            }
-            __syncwarp();
-            if (wl == 0) mbar_arrive(&S.x_empty);
+          tc_fence_before();
+          __syncwarp();
+          if (wl == 0) mbar_arrive(&S.x_full);
+          ok = ca_wait(&S.x_empty, x_phase);
+        } else {
+          ok = ca_wait(&S.x_full, x_phase);
+          tc_fence_after();
+          if (s.units > 1) {
+            const float ref1 = S.x_ref[lane_row], top = max3(ref, ref1, ref1);
+            mine = ref == -INFINITY ? 0.f : ex2(ref - top);
+            other = ref1 == -INFINITY ? 0.f : ex2(ref1 - top);
+            sum = sum * mine + S.x_sum[lane_row] * other;
+            ref = top;
           }
-          x_phase ^= 1;
-          if (!ok) break;
         }
+        x_phase ^= 1;
         if (!ok) break;
       }
-      if (w.one) load_queries(sn, wn);
+      // the next run's queries: all scores of this one are done
+      load_queries(sn, wn, s.units == 0);
       if (w.work && (!w.one || tl == 0)) {
         // ---- out, or the part of a split work tile
         const bool whole = s.begins && s.ends;
@@ -959,14 +995,24 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         const float inv = total == 0.f ? 0.f : 1.f / total;
         float* part = a.part_data + (size_t)(2 * blockIdx.x + (s.begins ? 1 : 0)) * kCaPartFloats;
         float probe = 0.f;  // NaN once a value is not finite
-        uint32_t o[2][32];
-        tmem_ld32(o_at, o[0]);
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
-          uint32_t* v = o[i & 1];
-          tmem_wait_ld();
-          tmem_tie32(v);
-          if (i < 3) tmem_ld32(o_at + (i + 1) * 32, o[(i + 1) & 1]);
+          uint32_t v[32];
+          tmem_ld32(o_at + i * 32, v);
+          if (w.one && s.units > 1) {
+            uint32_t o1[32];
+            tmem_ld32(o_at + 128 + i * 32, o1);
+            tmem_wait_ld();
+            tmem_tie32(v);
+            tmem_tie32(o1);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              v[e] = __float_as_uint(
+                  fmaf(__uint_as_float(o1[e]), other, __uint_as_float(v[e]) * mine));
+          } else {
+            tmem_wait_ld();
+            tmem_tie32(v);
+          }
 #pragma unroll
           for (int e = 0; e < 32; ++e) probe = fmaf(__uint_as_float(v[e]), 0.f, probe);
           if (!w.live) continue;
@@ -1021,6 +1067,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           }
         }
       }
+      if (w.one && tl == 0 && s.units > 0) {  // both groups' O have been read
+        tc_fence_before();
+        __syncwarp();
+        if (wl == 0) mbar_arrive(&S.x_empty);
+      }
+      if (sn.units == 0) break;
       s = sn;
       w = wn;
     }
@@ -1115,7 +1167,8 @@ cudaError_t launch_chunk_attn(const ChunkAttnRequest& r, int device, cudaStream_
   const uint64_t rows = uint64_t(r.num_blocks) * r.n_kv * r.block_size;
   CUtensorMap tmK, tmV;
   // a copy never leaves its page: the largest power of two that divides the page, 8 rows where
-  // only the whole lane is contiguous
+  // only the whole lane is contiguous (pages of 64, 4096 rows over 12288 positions: boxes of 64
+  // rows 443 us, of 16 446)
   const bool odd = r.block_size % 8 != 0;
   int box = 8;
   while (!odd && box < kCaKeys && r.block_size % (2 * box) == 0) box *= 2;

@@ -167,6 +167,17 @@ def test_chunk_attention_many_lanes(tt):
     check_attention(tt, q, b)
 
 
+@pytest.mark.parametrize("gqa,q32,seed", [(2, False, 41), (2, True, 42), (8, False, 43)])
+def test_chunk_attention_runs_of_every_kind(tt, gqa, q32, seed):
+    """Single rows, a few rows, one query tile, two and several, of one unit or more, in any order."""
+    rng = np.random.default_rng(seed)
+    new = rng.choice([1, 1, 2, 4, 5, 15, 17, 33, 64, 70, 129, 0], 400)
+    held = rng.choice([0, 0, 3, 60, 130, 300], 400)
+    b = ck.batch(seed, new, held, 2, 16)
+    q = rng.standard_normal((int(b[0][-1]), 2 * gqa, 128))
+    check_attention(tt, q.astype(np.float32 if q32 else np.float16), b)
+
+
 def test_chunk_attention_pages_outside_pool(tt):
     b = ck.batch(11, [9, 40], [70, 30], 2, 16)
     starts, spans, table, k, v = b
