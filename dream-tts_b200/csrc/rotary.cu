@@ -127,9 +127,15 @@ struct RotaryArgs {
   int* err;
 };
 
-// heads of one slot a thread takes at once: 128 bytes
+// Heads whose slots a thread has on their way at once. Plain rotation 4 of f16, 2 of f32 (64 bytes;
+// 12345 rows of 20 f16 heads of 96: 18.5 us, one head 24.3, 8 heads 21.5).
 template <typename T>
-constexpr int kRotHeads = 16 / int(sizeof(T));
+constexpr int kRotHeads = 8 / int(sizeof(T));
+// The append: 8 of f16, 2 of f32, whose sum of squares and norms take more registers (about 10k
+// rows of 36 f16 heads: 8 heads 18.7 us, 4 20.2, one 22.3; of 32 f32 heads: 2 heads 37.5 us, 4
+// 38.3, one 44.1).
+template <typename T>
+constexpr int kAppendHeads = sizeof(T) == 2 ? 8 : 2;
 
 // A CTA takes `tile` rows; a thread a row's slot in kRotHeads heads, `per` = ceil(heads /
 // that) heads apart (neighbouring threads read neighbouring slots and heads).
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a,
 }
 
 // `wpr` warps a row (1, 2, 4 or 8: more where rows are few), half a warp a head (16 slots of 8
-// dims, so the QK-norm's sum of squares is four exchanges), kRotHeads of them at once; warps take
+// dims, so the QK-norm's sum of squares is four exchanges), kAppendHeads of them at once; warps take
 // pairs of heads in turn.
 template <typename TX, typename TQ, bool kInter>
 __global__ void __launch_bounds__(kRotThreads, 3) rotary_append_kernel(const RotaryAppendRequest a,
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_append_kernel(const Rot
   const int all = a.heads + 2 * a.n_kv;
   const Slot s = slot_of(j, a.rotary, kInter);
   const long cap = (long)a.max_blocks * a.block_size;
-  constexpr int kHeads = kRotHeads<TX>;
+  constexpr int kHeads = kAppendHeads<TX>;
   for (int row = starts[0] + blockIdx.x * rows_at_once + (t >> 5) / wpr; row < starts[a.lanes];
        row += gridDim.x * rows_at_once) {
     const TX* src = static_cast<const TX*>(a.x) + (size_t)row * all * 128;
