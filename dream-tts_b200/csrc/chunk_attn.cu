@@ -60,52 +60,63 @@ TTS_DEV uint32_t ca_at(int r, int piece) {  // byte offset of 16-byte piece 0..1
          (uint32_t((piece & 7) ^ (r & 7)) << 4);
 }
 
+// kN bytes from global to shared memory, zeros unless `any`, asynchronously.
+template <int kN>
+TTS_DEV void ca_copy(void* to, const void* from, bool any) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(to)), "l"(from),
+               "n"(kN), "r"(any ? kN : 0)
+               : "memory");
+}
+TTS_DEV void ca_copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // The warp's 32 query rows (`rh`: each lane's row of q [rows * heads][128], -1: zeros) into rows
 // r0 .. r0 + 31 of the tile: half a warp a row of f16, a warp a row of f32, which is split into two
-// f16 pieces (22 bits) so that the scores keep f32 queries' precision.
+// f16 pieces (22 bits) so that the scores keep f32 queries' precision. A lane's f32 come to lie
+// where its own pieces go. (All copies are on their way at once in a short loop: loads to registers
+// took as long again to fetch their unrolled instructions as to arrive.)
 TTS_DEV uint32_t ca_sign(uint32_t two_halves, int negate) {
   return negate ? two_halves ^ 0x80008000u : two_halves;
 }
 TTS_DEV void ca_load_q(uint8_t (*tile)[kCaTileBytes], const __half* q, int rh, int r0, int negate) {
   const int wl = threadIdx.x & 31, sub = wl >> 4, e = wl & 15;
-  uint4 x[16];
-#pragma unroll
+#pragma unroll 2
   for (int k = 0; k < 16; ++k) {
     const int at = __shfl_sync(0xffffffffu, rh, 2 * k + sub);
-    x[k] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(q + (size_t)at * 128) + e)
-                   : make_uint4(0, 0, 0, 0);
+    ca_copy<16>(&tile[0][ca_at(r0 + 2 * k + sub, e)], q + (size_t)max(at, 0) * 128 + e * 8,
+                at >= 0);
   }
-#pragma unroll
-  for (int k = 0; k < 16; ++k)
-    *reinterpret_cast<uint4*>(&tile[0][ca_at(r0 + 2 * k + sub, e)]) =
-        make_uint4(ca_sign(x[k].x, negate), ca_sign(x[k].y, negate), ca_sign(x[k].z, negate),
-                   ca_sign(x[k].w, negate));
+  ca_copy_wait();
+  if (!negate) return;
+#pragma unroll 1
+  for (int k = 0; k < 16; ++k) {
+    uint4* x = reinterpret_cast<uint4*>(&tile[0][ca_at(r0 + 2 * k + sub, e)]);
+    *x = make_uint4(ca_sign(x->x, 1), ca_sign(x->y, 1), ca_sign(x->z, 1), ca_sign(x->w, 1));
+  }
 }
 TTS_DEV void ca_load_q(uint8_t (*tile)[kCaTileBytes], const float* q, int rh, int r0, int negate) {
   const int wl = threadIdx.x & 31;
-#pragma unroll
-  for (int k0 = 0; k0 < 32; k0 += 16) {
-    float4 x[16];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const int at = __shfl_sync(0xffffffffu, rh, k0 + k);
-      x[k] = at >= 0 ? __ldg(reinterpret_cast<const float4*>(q + (size_t)at * 128) + wl)
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const __half2 h0 = __floats2half2_rn(x[k].x, x[k].y), h1 = __floats2half2_rn(x[k].z, x[k].w);
-      const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-      const __half2 l0 = __floats2half2_rn(x[k].x - b0.x, x[k].y - b0.y),
-                    l1 = __floats2half2_rn(x[k].z - b1.x, x[k].w - b1.y);
-      const uint32_t to = ca_at(r0 + k0 + k, wl >> 1) + (wl & 1) * 8;
-      *reinterpret_cast<uint2*>(&tile[0][to]) =
-          make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&h0), negate),
+  const auto place = [&](int k) { return ca_at(r0 + k, wl >> 1) + (wl & 1) * 8; };
+#pragma unroll 2
+  for (int k = 0; k < 32; ++k) {
+    const int at = __shfl_sync(0xffffffffu, rh, k);
+    const float* from = q + (size_t)max(at, 0) * 128 + wl * 4;
+    ca_copy<8>(&tile[0][place(k)], from, at >= 0);
+    ca_copy<8>(&tile[1][place(k)], from + 2, at >= 0);
+  }
+  ca_copy_wait();
+#pragma unroll 4
+  for (int k = 0; k < 32; ++k) {
+    uint2 *hi = reinterpret_cast<uint2*>(&tile[0][place(k)]),
+          *lo = reinterpret_cast<uint2*>(&tile[1][place(k)]);
+    const float2 x = *reinterpret_cast<const float2*>(hi), y = *reinterpret_cast<const float2*>(lo);
+    const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(y.x, y.y);
+    const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+    const __half2 l0 = __floats2half2_rn(x.x - b0.x, x.y - b0.y),
+                  l1 = __floats2half2_rn(y.x - b1.x, y.y - b1.y);
+    *hi = make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&h0), negate),
                      ca_sign(*reinterpret_cast<const uint32_t*>(&h1), negate));
-      *reinterpret_cast<uint2*>(&tile[1][to]) =
-          make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&l0), negate),
+    *lo = make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&l0), negate),
                      ca_sign(*reinterpret_cast<const uint32_t*>(&l1), negate));
-    }
   }
 }
 
@@ -420,21 +431,25 @@ TTS_DEV void ca_plan(Smem& S, const CaArgs& a) {
     }
     return u;
   };
+  bool longer = false;
   for (int i = t; i < r.lanes; i += kCaThreads) {  // a thread a lane, if it has few work tiles
     const CaLane l = ca_lane(r, i);
     rows[i] = l.n;
     pos0[i] = l.pos0;
-    tot[i] = ca_tiles(l.n, r.gqa) <= 4 ? lane_units(l.n, l.pos0, 0, 1) * r.n_kv : -1;
+    const bool few = ca_tiles(l.n, r.gqa) <= 4;
+    tot[i] = few ? lane_units(l.n, l.pos0, 0, 1) * r.n_kv : -1;
+    longer = longer || !few;
   }
-  __syncthreads();
-  for (int i = warp; i < r.lanes; i += kCaThreads / 32) {  // a warp a longer one
-    if (tot[i] >= 0) continue;
-    long long u = lane_units(rows[i], pos0[i], wl, 32);
+  if (__syncthreads_or(longer)) {
+    for (int i = warp; i < r.lanes; i += kCaThreads / 32) {  // a warp a longer one
+      if (tot[i] >= 0) continue;
+      long long u = lane_units(rows[i], pos0[i], wl, 32);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    if (wl == 0) tot[i] = u * r.n_kv;
+      for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+      if (wl == 0) tot[i] = u * r.n_kv;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (warp == 0) {
     const auto before = [&](long long mine) {  // the sum over lower warp lanes
       long long inc = mine;
