@@ -27,13 +27,14 @@
 // for it after the first units), so no maximum is looked for in most units. Weights keep f16's 11
 // bits down to 2^-22 of r's; sums are f32.
 //
-// Measured (16 q heads, 8 kv heads): 4096 new rows over 12288 positions 439 us, 1096 TFLOP/s, 63 %
-// of the rate of a large plain product: a unit of two query tiles takes about 3.9k clocks, its MMAs
-// 2.4k to 2.9k and its exponentials 2.0k (16 a clock) of them, the rest is their hand-overs. 48
-// single rows over 4300 positions 148 us, 5.7 TB/s, 88 % of a copy: bound by HBM. 448 single rows
-// over 300: 197 us, 2.8 TB/s: a run of three units is too short to hide its start and end (210 us
-// with the queries loaded between runs, by the softmax warps; 325 with loops over a unit unrolled
-// and three copies of the loading code besides: instruction fetch).
+// Measured (16 q heads, 8 kv heads): 4096 new rows over 12288 positions 435 us, 1106 TFLOP/s, 64 %
+// of a large plain product's rate: a unit of two query tiles takes about 3.9k clocks, its MMAs 2.4k
+// to 2.9k and its exponentials 2.0k (16 a clock) of them, the rest is their hand-overs. With f32
+// queries 553 us: the scores are two products. 48 single rows over 4300 positions 148 us, 5.7 TB/s,
+// 88 % of a copy: bound by HBM. 448 single rows over 300: 184 us, 3.0 TB/s, and 592 chunks of 128
+// rows 41 us: runs of one to three units are too short to hide their start and end (about 10k
+// clocks). There the fetch of instructions counts, so loops over a unit stay rolled and queries
+// come by copies in short loops: unrolled, those two took 325 and 54 us.
 #include <mutex>
 
 #include "chunk_batch.cuh"
@@ -60,31 +61,31 @@ TTS_DEV uint32_t ca_at(int r, int piece) {  // byte offset of 16-byte piece 0..1
          (uint32_t((piece & 7) ^ (r & 7)) << 4);
 }
 
-// kN bytes from global to shared memory, zeros unless `any`, asynchronously.
-template <int kN>
+// 16 bytes from global to shared memory, zeros unless `any`, asynchronously.
 TTS_DEV void ca_copy(void* to, const void* from, bool any) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(to)), "l"(from),
-               "n"(kN), "r"(any ? kN : 0)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from),
+               "r"(any ? 16 : 0)
                : "memory");
 }
 TTS_DEV void ca_copy_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
-// The warp's 32 query rows (`rh`: each lane's row of q [rows * heads][128], -1: zeros) into rows
-// r0 .. r0 + 31 of the tile: half a warp a row of f16, a warp a row of f32, which is split into two
-// f16 pieces (22 bits) so that the scores keep f32 queries' precision. A lane's f32 come to lie
-// where its own pieces go. (All copies are on their way at once in a short loop: loads to registers
-// took as long again to fetch their unrolled instructions as to arrive.)
 TTS_DEV uint32_t ca_sign(uint32_t two_halves, int negate) {
   return negate ? two_halves ^ 0x80008000u : two_halves;
 }
-TTS_DEV void ca_load_q(uint8_t (*tile)[kCaTileBytes], const __half* q, int rh, int r0, int negate) {
+// The warp's 32 query rows (`rh`: each lane's row of q [rows * heads][128], -1: zeros) on their way
+// to rows r0 .. r0 + 31 of the tile (copies in a short loop: unrolled loads to registers took
+// longer to fetch their instructions than to arrive), and what is to be done once they are there.
+// Half a warp takes a row of f16, a warp a row of f32, which is split into two f16 pieces (22 bits)
+// so that the scores keep f32 queries' precision.
+TTS_DEV void ca_copy_q(uint8_t (*tile)[kCaTileBytes], const __half* q, int rh, int r0) {
   const int wl = threadIdx.x & 31, sub = wl >> 4, e = wl & 15;
 #pragma unroll 2
   for (int k = 0; k < 16; ++k) {
     const int at = __shfl_sync(0xffffffffu, rh, 2 * k + sub);
-    ca_copy<16>(&tile[0][ca_at(r0 + 2 * k + sub, e)], q + (size_t)max(at, 0) * 128 + e * 8,
-                at >= 0);
+    ca_copy(&tile[0][ca_at(r0 + 2 * k + sub, e)], q + (size_t)max(at, 0) * 128 + e * 8, at >= 0);
   }
+}
+TTS_DEV void ca_take_q(uint8_t (*tile)[kCaTileBytes], const __half*, int r0, int negate) {
+  const int wl = threadIdx.x & 31, sub = wl >> 4, e = wl & 15;
   ca_copy_wait();
   if (!negate) return;
 #pragma unroll 1
@@ -93,30 +94,39 @@ TTS_DEV void ca_load_q(uint8_t (*tile)[kCaTileBytes], const __half* q, int rh, i
     *x = make_uint4(ca_sign(x->x, 1), ca_sign(x->y, 1), ca_sign(x->z, 1), ca_sign(x->w, 1));
   }
 }
-TTS_DEV void ca_load_q(uint8_t (*tile)[kCaTileBytes], const float* q, int rh, int r0, int negate) {
+// A lane's four f32 wait in the 16 bytes of either tile where its and its neighbour's pieces go.
+TTS_DEV void ca_copy_q(uint8_t (*tile)[kCaTileBytes], const float* q, int rh, int r0) {
   const int wl = threadIdx.x & 31;
-  const auto place = [&](int k) { return ca_at(r0 + k, wl >> 1) + (wl & 1) * 8; };
 #pragma unroll 2
   for (int k = 0; k < 32; ++k) {
     const int at = __shfl_sync(0xffffffffu, rh, k);
-    const float* from = q + (size_t)max(at, 0) * 128 + wl * 4;
-    ca_copy<8>(&tile[0][place(k)], from, at >= 0);
-    ca_copy<8>(&tile[1][place(k)], from + 2, at >= 0);
+    ca_copy(&tile[wl & 1][ca_at(r0 + k, wl >> 1)], q + (size_t)max(at, 0) * 128 + wl * 4, at >= 0);
   }
+}
+TTS_DEV void ca_take_q(uint8_t (*tile)[kCaTileBytes], const float*, int r0, int negate) {
+  const int wl = threadIdx.x & 31;
   ca_copy_wait();
-#pragma unroll 4
-  for (int k = 0; k < 32; ++k) {
-    uint2 *hi = reinterpret_cast<uint2*>(&tile[0][place(k)]),
-          *lo = reinterpret_cast<uint2*>(&tile[1][place(k)]);
-    const float2 x = *reinterpret_cast<const float2*>(hi), y = *reinterpret_cast<const float2*>(lo);
-    const __half2 h0 = __floats2half2_rn(x.x, x.y), h1 = __floats2half2_rn(y.x, y.y);
-    const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-    const __half2 l0 = __floats2half2_rn(x.x - b0.x, x.y - b0.y),
-                  l1 = __floats2half2_rn(y.x - b1.x, y.y - b1.y);
-    *hi = make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&h0), negate),
+#pragma unroll 1
+  for (int k0 = 0; k0 < 32; k0 += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      x[k] = *reinterpret_cast<const float4*>(&tile[wl & 1][ca_at(r0 + k0 + k, wl >> 1)]);
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __half2 h0 = __floats2half2_rn(x[k].x, x[k].y), h1 = __floats2half2_rn(x[k].z, x[k].w);
+      const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+      const __half2 l0 = __floats2half2_rn(x[k].x - b0.x, x[k].y - b0.y),
+                    l1 = __floats2half2_rn(x[k].z - b1.x, x[k].w - b1.y);
+      const uint32_t to = ca_at(r0 + k0 + k, wl >> 1) + (wl & 1) * 8;
+      *reinterpret_cast<uint2*>(&tile[0][to]) =
+          make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&h0), negate),
                      ca_sign(*reinterpret_cast<const uint32_t*>(&h1), negate));
-    *lo = make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&l0), negate),
+      *reinterpret_cast<uint2*>(&tile[1][to]) =
+          make_uint2(ca_sign(*reinterpret_cast<const uint32_t*>(&l0), negate),
                      ca_sign(*reinterpret_cast<const uint32_t*>(&l1), negate));
+    }
   }
 }
 
@@ -344,16 +354,19 @@ TTS_DEV int ca_tiles(int n, int gqa) { return (n * gqa + kCaTile - 1) / kCaTile;
 
 struct CaLane {
   int row0, n, pos0;
+  bool bad;
 };
 // A lane's rows; a span the block table cannot hold leaves the lane without any.
-TTS_DEV CaLane ca_lane(const ChunkAttnRequest& r, int i) {
+TTS_DEV CaLane ca_lane(const ChunkAttnRequest& r, int start, int end, int span) {
   CaLane l;
-  l.row0 = r.row_start[i];
-  l.n = r.row_start[i + 1] - l.row0;
-  const int span = r.spans[i];
-  if (span < 0 || span > r.max_blocks * r.block_size) l.n = 0;
+  l.row0 = start;
+  l.bad = span < 0 || span > r.max_blocks * r.block_size;
+  l.n = l.bad ? 0 : end - start;
   l.pos0 = span - l.n;
   return l;
+}
+TTS_DEV CaLane ca_lane(const ChunkAttnRequest& r, int i) {
+  return ca_lane(r, r.row_start[i], r.row_start[i + 1], r.spans[i]);
 }
 
 template <typename TQ>
@@ -414,14 +427,21 @@ __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, i
 }
 
 // The CTA's share of the work: all CTAs compute the same totals from the lanes' lengths. Uses the
-// (still empty) tile ring as scratch.
+// (still empty) tile ring as scratch. False where the row starts are not in order.
 template <typename Smem>
-TTS_DEV void ca_plan(Smem& S, const CaArgs& a) {
+TTS_DEV bool ca_plan(Smem& S, const CaArgs& a) {
   const int t = threadIdx.x, warp = t >> 5, wl = t & 31;
   const ChunkAttnRequest& r = a.r;
   int* rows = reinterpret_cast<int*>(S.ring[0]);          // [lanes] new rows
   int* pos0 = rows + kChunkMaxLanes;                      // [lanes] the first one's position
   long long* tot = reinterpret_cast<long long*>(pos0 + kChunkMaxLanes);  // [lanes] units
+  int* starts = reinterpret_cast<int*>(tot + kChunkMaxLanes);            // [lanes + 1]
+  for (int i = t; i <= r.lanes; i += kCaThreads) {
+    starts[i] = r.row_start[i];
+    if (i < r.lanes) pos0[i] = r.spans[i];
+  }
+  __syncthreads();
+  if (!__syncthreads_and(chunk_starts_ok(starts, r.lanes, r.rows, t, kCaThreads))) return false;
   const auto lane_units = [&](int n, int p, int from, int step) {
     long long u = 0;
     for (int k = from; k < ca_tiles(n, r.gqa); k += step) {
@@ -433,7 +453,8 @@ TTS_DEV void ca_plan(Smem& S, const CaArgs& a) {
   };
   bool longer = false;
   for (int i = t; i < r.lanes; i += kCaThreads) {  // a thread a lane, if it has few work tiles
-    const CaLane l = ca_lane(r, i);
+    const CaLane l = ca_lane(r, starts[i], starts[i + 1], pos0[i]);
+    if (l.bad && blockIdx.x == 0) atomicOr(r.err, kFlagSpanRange);
     rows[i] = l.n;
     pos0[i] = l.pos0;
     const bool few = ca_tiles(l.n, r.gqa) <= 4;
@@ -501,6 +522,7 @@ TTS_DEV void ca_plan(Smem& S, const CaArgs& a) {
     }
   }
   __syncthreads();
+  return true;
 }
 
 template <typename TQ, int kK, int kV, int kParts>
@@ -516,17 +538,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   const ChunkAttnRequest& r = a.r;
   pdl_launch_dependents();  // the join waits for this grid's end before it reads
   if (t < 2) a.parts[2 * blockIdx.x + t].valid = 0;
-  if (!__syncthreads_and(chunk_starts_ok(r.row_start, r.lanes, r.rows, t, kCaThreads))) {
-    if (t == 0 && blockIdx.x == 0) atomicOr(r.err, kFlagChunkStarts);
-    return;
+  // what does not need the plan goes first, while its loads are on their way
+  if (warp == 9) {
+    tmem_alloc(&S.tmem, 512);
+    tmem_relinquish();
   }
-  if (blockIdx.x == 0)
-    for (int i = t; i < r.lanes; i += kCaThreads)
-      if (r.spans[i] < 0 || r.spans[i] > r.max_blocks * r.block_size)
-        atomicOr(r.err, kFlagSpanRange);
-  ca_plan(S, a);
-  if (S.count == 0) return;
-  if (t == 0) {
+  if (t == kCaThreads - 32) {
     for (int i = 0; i < kK + kV; ++i) {
       mbar_init(&S.full[i], 1);
       mbar_init(&S.empty[i], 1);
@@ -552,15 +569,17 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  if (warp == 9) {
-    tmem_alloc(&S.tmem, 512);
-    tmem_relinquish();
-  }
+  const bool planned = ca_plan(S, a);
+  if (!planned && t == 0 && blockIdx.x == 0) atomicOr(r.err, kFlagChunkStarts);
   fence_proxy_async();  // the plan's scratch before the copies into the same memory
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = S.tmem;
+  if (!planned || S.count == 0) {
+    if (warp == 9) tmem_dealloc(tmem, 512);
+    return;
+  }
   bool ok = true;
   int seg_slot = 0;
   uint32_t seg_phase = 0;
@@ -595,11 +614,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       if (free >= 0) ok = ca_wait(&S.seg_done[free % kCaSegs], (free / kCaSegs) & 1);
       if (!ok) return;
       const int f = s.flat0 + wl;
-      ca_load_q(S.q[buf], static_cast<const TQ*>(r.q),
+      ca_copy_q(S.q[buf], static_cast<const TQ*>(r.q),
                 f < s.n * r.gqa ? (s.row0 + f / r.gqa) * (r.n_kv * r.gqa) + s.head * r.gqa +
                                       f % r.gqa
                                 : -1,
-                0, a.negate);  // (the tile's other rows' scores are not read)
+                0);  // (the tile's other rows' scores are not read)
+      ca_take_q(S.q[buf], static_cast<const TQ*>(r.q), 0, a.negate);
       fence_proxy_async();
       __syncwarp();
       if (wl < 4) mbar_arrive(&S.q_full[buf]);
@@ -630,13 +650,6 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           p.valid = 1;
         }
       }
-      // its queries, wanted in a few microseconds, into L2
-      const int lines = int(sizeof(TQ)) * r.gqa;  // of 128 bytes, per token and kv head
-      const int q0 = s.flat0 / r.gqa, q1 = min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
-      for (int e = wl; e < (q1 - q0) * lines; e += 32)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(
-            static_cast<const char*>(r.q) +
-            (((size_t)(s.row0 + q0 + e / lines) * r.n_kv + s.head) * lines + e % lines) * 128));
       ok = ca_wait(&S.seg_empty[seg_slot], seg_phase ^ 1);
       if (!ok) break;
       if (wl == 0) {
@@ -645,6 +658,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       }
       __syncwarp();
       if (++seg_slot == kCaSegs) seg_slot = 0, seg_phase ^= 1;
+      // its queries, wanted in a few microseconds, into L2
+      const int lines = int(sizeof(TQ)) * r.gqa;  // of 128 bytes, per token and kv head
+      const int q0 = s.flat0 / r.gqa, q1 = min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
+      for (int e = wl; i > 0 && e < (q1 - q0) * lines; e += 32)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(
+            static_cast<const char*>(r.q) +
+            (((size_t)(s.row0 + q0 + e / lines) * r.n_kv + s.head) * lines + e % lines) * 128));
       if (i > 0) load_queries(before, i - 1);
       if (s.units == 0 || !ok) break;
       before = s;
@@ -816,6 +836,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           if (elect_one()) {
 #pragma unroll
             for (int kk = kCaHalf / 16; kk < 8; ++kk) values(kk);
+            if (one || b == 1) umma_commit(&S.empty[kK + v_slot]);  // before the scores: sooner free
             if (more)
               scores(b, one ? buf : b, k_slot,
                      j + ahead == s.units - 1 && (one || b == 1) ? done : nullptr);
@@ -825,12 +846,11 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           __syncwarp();
         }
         if (!ok) break;
-        if (elect_one()) {
-          umma_commit(&S.empty[kK + v_slot]);
-          if (more) umma_commit(&S.empty[k_slot]);
+        if (more) {
+          if (elect_one()) umma_commit(&S.empty[k_slot]);
+          __syncwarp();
+          next_k();
         }
-        __syncwarp();
-        if (more) next_k();
         if (++v_slot == kV) v_slot = 0, v_phase ^= 1;
       }
     }
@@ -862,14 +882,6 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       w.lo = r.window > 0 ? max(0, w.pos + 1 - r.window) : 0;
       w.rh = w.live ? (s.row0 + tok) * (r.n_kv * r.gqa) + s.head * r.gqa + w.f % r.gqa : -1;
       return w;
-    };
-    const auto load_queries = [&](const CaSeg& s, const CaRow& w, bool first) {
-      if (s.units == 0 || (w.one && tl == 1) || (w.few && !first)) return;
-      ca_load_q(S.q[tl], static_cast<const TQ*>(r.q), w.rh, (warp & 3) * 32, a.negate);
-      fence_proxy_async();
-      tc_fence_before();
-      __syncwarp();
-      if (wl == 0) mbar_arrive(&S.q_full[tl]);
     };
     CaSeg s{};
     CaRow w = rows_of(s);
@@ -969,7 +981,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       CaSeg sn{};
       ok = next_seg(&sn);
       if (!ok) break;
+      // The next run's queries, unless the walk loads them: this tile's scores are all done, of a
+      // lone tile the other group's may not be.
       const CaRow wn = rows_of(sn);
+      const bool load = sn.units > 0 && !(wn.one && tl == 1) && !(wn.few && s.units > 0);
+      if (load && !w.one)
+        ca_copy_q(S.q[tl], static_cast<const TQ*>(r.q), wn.rh, (warp & 3) * 32);
       if (step0 < s.units) {
         ok = ca_wait(&S.o_full[tl], o_phase);
         o_phase ^= 1;
@@ -1001,8 +1018,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         x_phase ^= 1;
         if (!ok) break;
       }
-      // the next run's queries: all scores of this one are done
-      load_queries(sn, wn, s.units == 0);
+      if (load) {
+        if (w.one) ca_copy_q(S.q[tl], static_cast<const TQ*>(r.q), wn.rh, (warp & 3) * 32);
+        ca_take_q(S.q[tl], static_cast<const TQ*>(r.q), (warp & 3) * 32, a.negate);
+        fence_proxy_async();
+        tc_fence_before();
+        __syncwarp();
+        if (wl == 0) mbar_arrive(&S.q_full[tl]);
+      }
       if (w.work && (!w.one || tl == 0)) {
         // ---- out, or the part of a split work tile
         const bool whole = s.begins && s.ends;
@@ -1092,7 +1115,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       w = wn;
     }
   }
-  if (!ok && wl == 0) atomicOr(r.err, kFlagAttnWait);
+  if (!ok) {
+    ca_copy_wait();
+    if (wl == 0) atomicOr(r.err, kFlagAttnWait);
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
