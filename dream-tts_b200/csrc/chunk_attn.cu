@@ -836,7 +836,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           if (elect_one()) {
 #pragma unroll
             for (int kk = kCaHalf / 16; kk < 8; ++kk) values(kk);
-            if (one || b == 1) umma_commit(&S.empty[kK + v_slot]);  // before the scores: sooner free
+            if (one || b == 1) umma_commit(&S.empty[kK + v_slot]);  // sooner than the scores
             if (more)
               scores(b, one ? buf : b, k_slot,
                      j + ahead == s.units - 1 && (one || b == 1) ? done : nullptr);

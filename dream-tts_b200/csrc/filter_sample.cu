@@ -11,11 +11,20 @@
 // and weights in 1024 bins of equal width in log w. A cut or the draw then falls into one bin,
 // found by a scan; only that bin's ids are gathered into the first CTA, sorted and walked. Where
 // the first filter leaves few ids, all of them are gathered at once and the rest happens there.
-// A bin with too many ids (equal logits) is narrowed by the bits of its keys.
+// A bin with too many ids (equal logits) is narrowed by the bits of its keys. Counts are kept only
+// where top-k asks for them.
 //
 // A weight is evaluated in 64 bits and held as an integer multiple of 2^-44: sums of up to 2^18
 // of them are exact in 64 bits, so neither the order of the atomics nor the number of CTAs can
 // change a pick.
+//
+// Measured (192 rows of 151851 f32 ids, top-p 0.9): 243 us; reading them once takes 18. What bounds
+// it is the chain of a row's steps (load, maximum, bins, exchange, cut, draw), each behind a
+// barrier of the CTA or cluster: issue slots are 41 % used, a row alone takes 31 us, and some 36
+// rows are at work at a time. So the row stays in shared memory, two CTAs share an SM, and CTAs
+// exchange little. (The bins cost 61 us of it in atomics and 47 besides; 512 of them 276 us, 2048
+// 247. Clusters of 16 CTAs 399 to 461.) 48 rows of 32003 with every filter 23 us, 8 rows of 2048
+// with top-k alone 10 us.
 #include <mutex>
 
 #include "tts_common.cuh"
@@ -29,12 +38,15 @@ typedef unsigned long long u64;
 constexpr int kFsThreads = 512;
 constexpr int kFsWarps = kFsThreads / 32;
 constexpr int kFsBins = 1024;
-constexpr int kFsLoads = 8;      // 16-byte loads a thread has on their way
+constexpr int kFsLoads = 4;      // 16-byte loads a thread has on their way
 constexpr int kFsCap = 1024;     // ids the first CTA sorts at once
-constexpr int kFsFew = 96;       // ... without looking closer first
+// ... without cutting the list into parts first (192 rows of 151851: 247 us, all sorted whole 287)
+constexpr int kFsFew = 96;
 constexpr int kFsMaxCluster = 8;
 constexpr float kFsOctaves = 45.f;  // below 2^-45 a weight is 0
-constexpr int kFsTwo = 19456;    // ids in a CTA's part up to which two CTAs share an SM
+// Ids in a CTA's part up to which two CTAs share an SM (192 rows of 151851: two 247 us, one with
+// twice the part 256; 512 rows of 32000: 129 and 136).
+constexpr int kFsTwo = 19456;
 constexpr double kFsOne = 17592186044416.0;  // 2^44: the weight of the row's maximum
 
 // Counts and 64-bit weights, the latter in two words each.
@@ -69,7 +81,7 @@ struct FsSmem {
   uint32_t mine;                // ids this CTA gathers
   int digit_at;                 // the part of the keys that a target falls into
   u64 digit_below[2];           // and the weight and count above it
-  alignas(16) float x[4];       // this CTA's part of the row (a.per entries), -inf: not to be picked
+  alignas(16) float x[4];       // this CTA's part of the row (a.per entries), -inf: never picked
 };
 
 // NaN is not to be picked, -0 is 0.
@@ -273,7 +285,8 @@ TTS_DEV void fs_sort(FsSmem& S, const FsScale& r, int m) {
     if (part == 0 && i < m) e[u] = S.list[i], at[u] = i;
     const u64 mine = i < m ? S.list[i] : ~0ull;
     int larger = 0;
-    const int from = part * each & ~1, to = part == parts - 1 ? pad : min(pad, (part + 1) * each & ~1);
+    const int from = part * each & ~1;
+    const int to = part == parts - 1 ? pad : min(pad, (part + 1) * each & ~1);
 #pragma unroll 4
     for (int j = from; j < to; j += 2) {
       const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(&S.list[j]);
@@ -613,7 +626,9 @@ __global__ void __launch_bounds__(kFsThreads, 2) filter_sample_kernel(const FsAr
 template <typename T>
 cudaError_t launch_as(const FilterSampleRequest& r, int device, cudaStream_t st) {
   // The fewest CTAs a row whose part of it leaves room for two of them on an SM, then twice as
-  // many while the rows do not fill the SMs and a part stays at 2048 ids or more.
+  // many while the rows do not fill the SMs and a part stays at 2048 ids or more (8 rows of 32000:
+  // 22.1 us, without that 28.4, down to 4096 only 23.7; 8 rows of 2048 in parts of 1024: 11.7 for
+  // 10.2).
   const int sms = num_sms(device);
   int ctas = 1;
   while (ctas < kFsMaxCluster &&

@@ -10,7 +10,12 @@
 // pairs: in the half layout slot j < r/8 is dims 4j..4j+3 and r/2 + 4j..+3, else 8 consecutive
 // dims. The work is one read and one write of the rows: bound by HBM. A thread keeps its slot
 // through several heads, so a row's table entries are read once for them, and has the heads' loads
-// on their way together.
+// on their way together. (The layout is a template parameter: values indexed by a run-time choice
+// of pairs went to local memory.)
+//
+// Measured: plain, 12345 rows of 20 f16 heads of 96 dims, tables of 131072 positions: 18.5 us (a
+// copy's rate: 15.0); 77 rows of 12 f32 heads: 2.2 us. Append: about 10k rows of 32 f32 heads with
+// norms 37.5 us (31.9); of 36 f16 heads, interleaved, 18.8 us (11.7); 48 rows 3.3 us.
 #include "chunk_batch.cuh"
 
 namespace tts {
@@ -176,9 +181,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotaryArgs a,
   }
 }
 
-// `wpr` warps a row (1, 2, 4 or 8: more where rows are few), half a warp a head (16 slots of 8
-// dims, so the QK-norm's sum of squares is four exchanges), kAppendHeads of them at once; warps take
-// pairs of heads in turn.
+// `wpr` warps a row (1, 2, 4 or 8), half a warp a head (16 slots of 8 dims, so the QK-norm's sum of
+// squares is four exchanges), kAppendHeads of them at once; warps take pairs of heads in turn.
 template <typename TX, typename TQ, bool kInter>
 __global__ void __launch_bounds__(kRotThreads, 3) rotary_append_kernel(const RotaryAppendRequest a,
                                                                     int wpr) {
@@ -288,7 +292,8 @@ cudaError_t launch_rotary(const void* x, bool f16, int rows, int heads, int hd, 
                           cudaStream_t st) {
   RotaryArgs a{x,     y,     rows,     heads,  hd,          ldx, ldy, positions,
                cos_t, sin_t, rope_len, rotary, interleaved, err};
-  // rows a CTA: enough to give each thread an item, at most 8
+  // rows a CTA: enough to give each thread an item, at most 8 (12345 rows of 20 f16 heads of 96: 8
+  // rows 21.5 us, one row 36.6)
   const int at_once = f16 ? kRotHeads<__half> : kRotHeads<float>;
   const int items = (heads + at_once - 1) / at_once * (hd / 8);
   int tile = 1;
@@ -306,7 +311,8 @@ cudaError_t launch_rotary(const void* x, bool f16, int rows, int heads, int hd, 
 }
 
 cudaError_t launch_rotary_append(const RotaryAppendRequest& r, int device, cudaStream_t st) {
-  // as few warps a row as still fill the SMs (8 CTAs each)
+  // as few warps a row as still fill the SMs (8 CTAs each): rows of 32 f32 heads, 48 of them 3.3 us
+  // (a warp each 8.9), about 10k 37.5 us (8 warps each 56.7)
   const int sms = num_sms(device), full = sms * 8;
   int wpr = 1;
   while (wpr < 8 && (long)r.rows * wpr < (long)full * 8) wpr *= 2;
