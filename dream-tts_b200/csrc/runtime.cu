@@ -663,6 +663,11 @@ static tts_status chunk_ok(const char* op, const tts_chunk_batch* b, const tts_k
   return TTS_OK;
 }
 
+static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
+
 static tts_status rotary_ok(const char* op, int hd, int rope_len, int rotary, int interleaved,
                             const float* cos_t, const float* sin_t) {
   const std::string name = std::string(op) + ": ";
@@ -697,6 +702,16 @@ tts_status tts_rotary(tts_ctx* c, const void* x, int x_f16, int rows, int heads,
   if (!aligned16(x) || !aligned16(y))
     return fail(TTS_ERR_INVALID_ARG, "rotary: pointers must be 16-byte aligned");
   if (rows == 0) return TTS_OK;
+  const size_t size = x_f16 ? 2 : 4;
+  if (x != y && overlap(x, (size_t(rows - 1) * ldx + width) * size, y,
+                        (size_t(rows - 1) * ldy + width) * size)) {
+    // other columns of the same rows are fine
+    const size_t pitch = ldx * size, used = width * size;
+    const uintptr_t from = reinterpret_cast<uintptr_t>(x), to = reinterpret_cast<uintptr_t>(y);
+    const size_t off = (to > from ? to - from : from - to) % pitch;
+    if (ldx != ldy || off < used || off + used > pitch)
+      return fail(TTS_ERR_INVALID_ARG, "rotary: y must be x or lie apart from it");
+  }
   DeviceGuard g(c->device);
   return counted(launch_rotary(x, x_f16 != 0, rows, heads, head_dim, ldx, positions, cos_t, sin_t,
                                rope_len, rotary_dim, interleaved != 0, y, ldy, c->gemm.err,
@@ -719,6 +734,10 @@ tts_status tts_rotary_append(tts_ctx* c, const void* qkv, int qkv_f16, int heads
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(norms))
     return fail(TTS_ERR_INVALID_ARG, "rotary_append: pointers must be 16-byte aligned");
   if (b->rows == 0) return TTS_OK;
+  const size_t row = size_t(b->rows) * 128;
+  if (overlap(qkv, row * (heads + 2 * size_t(kv->n_kv)) * (qkv_f16 ? 2 : 4), q_out,
+              row * heads * (q_f16 ? 2 : 4)))
+    return fail(TTS_ERR_INVALID_ARG, "rotary_append: q must lie apart from qkv");
   DeviceGuard g(c->device);
   RotaryAppendRequest r;
   r.x = qkv;
@@ -772,6 +791,9 @@ tts_status tts_chunk_attention(tts_ctx* c, const void* q, int q_f16, int gqa,
   if (!workspace || workspace_bytes < chunk_attn_workspace(c->device))
     return fail(TTS_ERR_INVALID_ARG,
                 "chunk_attention: the workspace is smaller than tts_chunk_attention_workspace");
+  const size_t elems = size_t(b->rows) * kv->n_kv * gqa * 128;
+  if (overlap(q, elems * (q_f16 ? 2 : 4), out_f16, elems * 2))
+    return fail(TTS_ERR_INVALID_ARG, "chunk_attention: out must lie apart from q");
   DeviceGuard g(c->device);
   ChunkAttnRequest r;
   r.q = q;

@@ -74,6 +74,8 @@ def chunk_attention(q: torch.Tensor, row_start: torch.Tensor, spans: torch.Tenso
     rows, heads, _ = q.shape
     if heads % kv.n_kv:
         raise ValueError(f"chunk_attention: {heads} heads over {kv.n_kv} kv heads")
+    if not -2 ** 31 <= window < 2 ** 31:
+        raise ValueError("chunk_attention: window must be 0 or a number of positions below 2^31")
     same_device("chunk_attention", q, row_start, spans, out)
     b = chunk_batch("chunk_attention", rows, row_start, spans, kv)
     if out is None:

@@ -76,6 +76,7 @@ def chunk_batch(op: str, rows: int, row_start: torch.Tensor, spans: torch.Tensor
         raise ValueError(f"{op}: row_start must hold one entry more than spans, both contiguous")
     if lanes > getattr(kv, "lanes", lanes):
         raise ValueError(f"{op}: {lanes} lanes over a block table of {kv.lanes}")
+    same_device(op, row_start, *getattr(kv, "keep", ()))
     return L.ChunkBatch(lanes, rows, row_start.data_ptr(), spans.data_ptr())
 
 
@@ -96,8 +97,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
            interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Rotary positions on `x [rows, heads, head_dim]` (f32 or f16), row r at `positions[r]`
     (int32): the first 2 * cos.shape[1] dims of each head in half-split or interleaved pairs, the
-    rest copied. x may be a column block of wider rows. Into `out` (may be x), else a new
-    tensor."""
+    rest copied. x may be a column block of wider rows. Into `out` (x, or memory
+    apart from it), else a new tensor."""
     if x.dim() != 3 or x.dtype not in (torch.float32, torch.float16):
         raise ValueError("rotary: x must be [rows, heads, head_dim], f32 or f16")
     rows, heads, hd = x.shape
@@ -154,7 +155,7 @@ def rotary_append(qkv: torch.Tensor, heads: int, row_start: torch.Tensor, spans:
     x = qkv.contiguous()
     nm = None if norms is None else as_type(norms, torch.float32)
     L.call("tts_rotary_append", ctx_of(x), x.data_ptr(), int(x.dtype == torch.float16), int(heads),
-           C.byref(b), None if nm is None else nm.data_ptr(), float(eps), c.data_ptr(), s.data_ptr(), c.shape[0],
-           2 * c.shape[1], int(interleaved), C.byref(kv), q.data_ptr(),
+           C.byref(b), None if nm is None else nm.data_ptr(), float(eps), c.data_ptr(),
+           s.data_ptr(), c.shape[0], 2 * c.shape[1], int(interleaved), C.byref(kv), q.data_ptr(),
            int(q.dtype == torch.float16), stream_of(x))
     return q

@@ -269,9 +269,9 @@ typedef struct tts_chunk_batch {
 
 /* Rotary positions (candle_nn::rotary_emb, rope and rope_i): rows of x [rows][heads][head_dim],
  * f32 or f16, `ldx` elements from row to row (0: heads * head_dim), row r at positions[r]
- * (device), into y of the same type (may be x itself). Pair (a, b) becomes (a cos - b sin,
- * b cos + a sin); pairs are dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved = 1,
- * of the first rotary_dim dims of a head, the rest is copied. cos/sin f32
+ * (device), into y of the same type (x itself or apart from it). Pair (a, b) becomes
+ * (a cos - b sin, b cos + a sin); pairs are dims (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with
+ * interleaved = 1, of the first rotary_dim dims of a head, the rest is copied. cos/sin f32
  * [rope_len][rotary_dim / 2], scaled for long contexts by whoever makes them. head_dim <= 256,
  * head_dim and rotary_dim multiples of 8, strides too. A position outside the tables skips its
  * row and is reported by tts_ctx_check. */
@@ -282,9 +282,9 @@ TTS_API tts_status tts_rotary(tts_ctx* ctx, const void* x, int x_f16, int rows, 
 
 /* tts_qk_rope_append for a ragged chunk: qkv f32 or f16 [rows][(heads + 2 n_kv) * 128]; the
  * QK-norm when `norms` is given (f32 [2][128], q's then k's weight, over the whole head), then
- * the rotation of tts_rotary at each row's position; q f32 or f16 [rows][heads][128] out, K and
- * V (f16) into the pages (any page size). A position outside the tables or a page outside the
- * pool skips its row and is reported by tts_ctx_check. */
+ * the rotation of tts_rotary at each row's position; q f32 or f16 [rows][heads][128] out (apart
+ * from qkv), K and V (f16) into the pages (any page size). A position outside the tables or a
+ * page outside the pool skips its row and is reported by tts_ctx_check. */
 TTS_API tts_status tts_rotary_append(tts_ctx* ctx, const void* qkv, int qkv_f16, int heads,
                                      const tts_chunk_batch* batch, const float* norms, float eps,
                                      const float* cos_t, const float* sin_t, int rope_len,
@@ -293,10 +293,10 @@ TTS_API tts_status tts_rotary_append(tts_ctx* ctx, const void* qkv, int qkv_f16,
 
 /* Attention of a ragged chunk over its lanes' pages, its own K and V rows included: the row at
  * position p sees positions max(0, p + 1 - window) .. p (window 0: 0 .. p), scores q.k * scale.
- * q f32 or f16 [rows][n_kv * gqa][128], out f16 of the same shape; gqa 1..16; block_size a
- * multiple of 8 unless max_blocks == 1. A row that sees no position (more new rows than spans
- * says) is 0, and what the pages hold at positions a row does not see never reaches it. Pages
- * outside the pool read as zero and are reported by tts_ctx_check. `workspace` (device,
+ * q f32 or f16 [rows][n_kv * gqa][128], out f16 of the same shape (apart from q); gqa 1..16;
+ * block_size a multiple of 8 unless max_blocks == 1. A row that sees no position (more new rows
+ * than spans says) is 0, and what the pages hold at positions a row does not see never reaches it.
+ * Pages outside the pool read as zero and are reported by tts_ctx_check. `workspace` (device,
  * tts_chunk_attention_workspace bytes for any call on the context's device, contents of no
  * meaning before or after) belongs to the call until it ends on the GPU: calls that may overlap
  * need one each. */

@@ -117,6 +117,32 @@ def test_scaled_tables():
     assert all(np.abs(a.numpy() - b.numpy()).max() <= 2.0 ** -23 for a, b in zip(same, ref))
 
 
+def test_overlapping_buffers_are_refused(lib):
+    """Outputs over inputs that other blocks may still read."""
+    for f16, out in ((1, A), (1, A + 8 * 4 * 256 - 16), (0, A + 8 * 4 * 512 - 16)):
+        refused(lib, 1, "apart from q", "tts_chunk_attention", CTX, A, f16, 2, lanes(), kv(), 1.0, 0, out, A,
+                1 << 40, None)
+    for q in (A, A + 8 * 8 * 512 - 16, A - 16):
+        refused(lib, 1, "apart from qkv", "tts_rotary_append", CTX, A, 0, 4, lanes(), None, 1e-6, A, A, 64, 64, 0,
+                kv(), q, 0, None)
+    for y, ld in ((A + 16, 0), (A + 512, 0), (A + 16, 256), (A + 512 - 16, 256), (A + 1024 - 16, 256)):
+        refused(lib, 1, "apart from it", "tts_rotary", CTX, A, 0, 3, 2, 64, ld, A, A, A, 10, 64, 0, y, ld, None)
+
+
+def test_cache_on_another_device_is_refused():
+    import torch
+    at = lambda *shape, dtype=torch.float16: torch.zeros(*shape, dtype=dtype, device="meta")
+    cache = ttsnn.attn.paged_cache(at(4, 2, 8, 128), at(4, 2, 8, 128), at(1, 4, dtype=torch.int32))
+    starts, spans = torch.tensor([0, 2], dtype=torch.int32), torch.tensor([3], dtype=torch.int32)
+    with pytest.raises(ValueError, match="meta"):
+        ttsnn.attn.chunk_attention(torch.zeros(2, 4, 128), starts, spans, cache, 1.0)
+    with pytest.raises(ValueError, match="meta"):
+        ttsnn.qkrope.rotary_append(torch.zeros(2, 1024), 4, starts, spans, torch.zeros(8, 64),
+                                   torch.zeros(8, 64), cache)
+    with pytest.raises(ValueError, match="2\\^31"):
+        ttsnn.attn.chunk_attention(torch.zeros(2, 4, 128), starts, spans, cache, 1.0, window=2 ** 32 + 5)
+
+
 @pytest.mark.parametrize("kw", [dict(kind="other"), dict(kind="yarn"), dict(factor=0.0), dict(rotary_dim=7),
                                 dict(length=0), dict(kind="ntk", rotary_dim=2),
                                 dict(kind="yarn", original=100, beta_fast=1.0)])

@@ -268,6 +268,17 @@ def test_rotary(tt, hd, rotary, interleaved, f16):
     tt.check()
 
 
+def test_rotary_into_other_columns_of_the_same_rows(tt):
+    rng = np.random.default_rng(51)
+    wide = dev(rng.standard_normal((37, 2, 3, 64)).astype(np.float32))
+    pos, (cos, sin) = dev(rng.integers(0, 90, 37).astype(np.int32)), (dev(t) for t in ck.tables(90, 64))
+    before = wide[:, 0].clone()
+    want = tt.qkrope.rotary(before, pos, cos, sin)
+    tt.qkrope.rotary(wide[:, 0], pos, cos, sin, out=wide[:, 1])
+    tt.check()
+    assert torch.equal(wide[:, 0], before) and torch.equal(wide[:, 1], want)
+
+
 def test_rotary_positions_outside_the_tables(tt):
     cos, sin = ck.tables(10, 16)
     x = dev(np.ones((4, 2, 16), np.float32))
