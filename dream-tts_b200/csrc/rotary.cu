@@ -14,8 +14,8 @@
 // of pairs went to local memory.)
 //
 // Measured: plain, 12345 rows of 20 f16 heads of 96 dims, tables of 131072 positions: 18.5 us (a
-// copy's rate: 15.0); 77 rows of 12 f32 heads: 2.2 us. Append: about 10k rows of 32 f32 heads with
-// norms 37.5 us (31.9); of 36 f16 heads, interleaved, 18.8 us (11.7); 48 rows 3.3 us.
+// copy's rate: 15.0); 77 rows of 12 f32 heads: 2.2 us. Append: about 8k rows of 32 f32 heads with
+// norms 37.5 us (31.9); 4k of 36 f16 heads, interleaved, 18.8 us (11.7); 48 rows 3.3 us.
 #include "chunk_batch.cuh"
 
 namespace tts {
@@ -136,8 +136,8 @@ struct RotaryArgs {
 // 12345 rows of 20 f16 heads of 96: 18.5 us, one head 24.3, 8 heads 21.5).
 template <typename T>
 constexpr int kRotHeads = 8 / int(sizeof(T));
-// The append: 8 of f16, 2 of f32, whose sum of squares and norms take more registers (about 10k
-// rows of 36 f16 heads: 8 heads 18.7 us, 4 20.2, one 22.3; of 32 f32 heads: 2 heads 37.5 us, 4
+// The append: 8 of f16, 2 of f32, whose sum of squares and norms take more registers (about 4k
+// rows of 36 f16 heads: 8 heads 18.7 us, 4 20.2, one 22.3; 8k of 32 f32 heads: 2 heads 37.5 us, 4
 // 38.3, one 44.1).
 template <typename T>
 constexpr int kAppendHeads = sizeof(T) == 2 ? 8 : 2;
@@ -312,7 +312,7 @@ cudaError_t launch_rotary(const void* x, bool f16, int rows, int heads, int hd, 
 
 cudaError_t launch_rotary_append(const RotaryAppendRequest& r, int device, cudaStream_t st) {
   // as few warps a row as still fill the SMs (8 CTAs each): rows of 32 f32 heads, 48 of them 3.3 us
-  // (a warp each 8.9), about 10k 37.5 us (8 warps each 56.7)
+  // (a warp each 8.9), about 8k 37.5 us (8 warps each 56.7)
   const int sms = num_sms(device), full = sms * 8;
   int wpr = 1;
   while (wpr < 8 && (long)r.rows * wpr < (long)full * 8) wpr *= 2;
