@@ -182,13 +182,20 @@ struct CaPart {
 };
 constexpr int kCaPartFloats = kCaTile * 130;  // O [32][256] float4, m [256], l [256]
 
+// n / d for 0 <= n < 2^31: n m >> s, m = floor(2^s / d) + 1, s = 31 + ceil(log2 d) (Granlund and
+// Montgomery 1994). A division of its own is some twenty instructions to fetch.
+struct CaDiv {
+  uint32_t m, s;
+};
+TTS_DEV int operator/(int n, CaDiv d) { return int((uint64_t(uint32_t(n)) * d.m) >> d.s); }
+
 struct CaArgs {
   ChunkAttnRequest r;
   float c;      // |scale| log2 e
   int negate;   // scale < 0: the queries change sign
   int box;      // rows of a page that one copy takes
   int odd;      // one page per lane, of no multiple of 8 rows
-  uint32_t div_m, div_s;  // p / block_size = p * div_m >> 32 + div_s for 0 <= p < 2^31
+  CaDiv by_page, by_gqa;  // by block_size, by r.gqa
   int wide;     // out is 32-byte aligned: whole sectors at a time (4600 rows of 16 heads, in chunks
                 // of up to 701: 138 us, in halves 144)
   CaPart* parts;
@@ -343,7 +350,7 @@ TTS_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc
 }
 // First unit and number of units of a lane's work tile k (at least one: rows that see nothing are
 // written too).
-TTS_DEV void ca_units(int n, int pos0, int gqa, int window, int k, int* first, int* count) {
+TTS_DEV void ca_units(int n, int pos0, CaDiv gqa, int window, int k, int* first, int* count) {
   const int t0 = k * kCaTile / gqa, t1 = min(n, (k * kCaTile + kCaTile - 1) / gqa + 1);
   const int lo = window > 0 ? max(0, pos0 + t0 + 1 - window) : 0;
   const int last = max(0, pos0 + t1 - 1) / kCaKeys;
@@ -391,7 +398,7 @@ template <typename TQ>
 __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, int hi, float ref,
                                        float4* o) {
   const int wl = threadIdx.x & 31;
-  const int tok = f / a.r.gqa, head = s.head * a.r.gqa + f % a.r.gqa;
+  const int tok = f / a.by_gqa, head = s.head * a.r.gqa + f - tok * a.r.gqa;
   const int pos = s.pos0 + tok;
   const int u0 = s.unit0 * kCaKeys, u1 = min(hi, (s.unit0 + s.units) * kCaKeys);
   const int lo = a.r.window > 0 ? max(0, pos + 1 - a.r.window) : 0;
@@ -446,7 +453,7 @@ TTS_DEV bool ca_plan(Smem& S, const CaArgs& a) {
     long long u = 0;
     for (int k = from; k < ca_tiles(n, r.gqa); k += step) {
       int first, count;
-      ca_units(n, p, r.gqa, r.window, k, &first, &count);
+      ca_units(n, p, a.by_gqa, r.window, k, &first, &count);
       u += count;
     }
     return u;
@@ -488,7 +495,8 @@ TTS_DEV bool ca_plan(Smem& S, const CaArgs& a) {
     for (int i = l0; i < l1; ++i) mine += tot[i];
     const long long pre = before(mine);
     const long long all = __shfl_sync(0xffffffffu, pre + mine, 31);
-    const long long per = (all + gridDim.x - 1) / gridDim.x;
+    const long long per = all <= INT_MAX ? (uint32_t(all) + gridDim.x - 1) / gridDim.x
+                                         : (all + gridDim.x - 1) / gridDim.x;
     const long long lo = per * blockIdx.x, hi = lo + per < all ? lo + per : all;
     if (wl == 0) S.count = lo < hi ? int(hi - lo) : 0;
     if (lo < hi) {
@@ -505,7 +513,7 @@ TTS_DEV bool ca_plan(Smem& S, const CaArgs& a) {
       const int n = rows[lane], p = pos0[lane], tiles = ca_tiles(n, r.gqa);
       for (int k0 = 0; k0 < tiles; k0 += 32) {
         int first = 0, count = 0;
-        if (k0 + wl < tiles) ca_units(n, p, r.gqa, r.window, k0 + wl, &first, &count);
+        if (k0 + wl < tiles) ca_units(n, p, a.by_gqa, r.window, k0 + wl, &first, &count);
         const long long here = (long long)count * r.n_kv, low = before(here);
         const unsigned m = __ballot_sync(0xffffffffu, rem >= low && rem < low + here);
         if (m) {
@@ -543,31 +551,18 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     tmem_alloc(&S.tmem, 512);
     tmem_relinquish();
   }
-  if (t == kCaThreads - 32) {
-    for (int i = 0; i < kK + kV; ++i) {
-      mbar_init(&S.full[i], 1);
-      mbar_init(&S.empty[i], 1);
+  if (warp == 11) {
+    for (uint64_t* b = S.full + wl; b <= &S.x_empty; b += 32) {
+      const auto one_of = [b](const uint64_t* s, int n) { return b >= s && b < s + n; };
+      const bool warps = one_of(S.q_full, 2) || one_of(S.h_full, 2) || one_of(S.p_full, 2) ||
+                         one_of(&S.x_full, 1) || one_of(&S.x_empty, 1);
+      mbar_init(b, warps ? 4 : one_of(S.seg_empty, kCaSegs) ? 11 : 1);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&S.q_full[i], 4);
-      mbar_init(&S.s_full[i], 1);
-      mbar_init(&S.h_full[i], 4);  // half of P
-      mbar_init(&S.h_done[i], 1);
-      mbar_init(&S.p_full[i], 4);
-      mbar_init(&S.o_full[i], 1);
-    }
-    for (int i = 0; i < kCaSegs; ++i) {
-      mbar_init(&S.seg_full[i], 1);
-      mbar_init(&S.seg_empty[i], 11);
-      mbar_init(&S.seg_done[i], 1);  // all its scores are
-    }
-    mbar_init(&S.x_full, 4);
-    mbar_init(&S.x_empty, 4);
-    mbar_init(&S.tail, 1);
-    mbar_init(&S.drain, 1);
     fence_barrier_init();
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
+    if (wl == 0) {
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+    }
   }
   const bool planned = ca_plan(S, a);
   if (!planned && t == 0 && blockIdx.x == 0) atomicOr(r.err, kFlagChunkStarts);
@@ -613,11 +608,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       if (!few || i == 0) return;
       if (free >= 0) ok = ca_wait(&S.seg_done[free % kCaSegs], (free / kCaSegs) & 1);
       if (!ok) return;
-      const int f = s.flat0 + wl;
+      const int f = s.flat0 + wl, tok = f / a.by_gqa;
       ca_copy_q(S.q[buf], static_cast<const TQ*>(r.q),
-                f < s.n * r.gqa ? (s.row0 + f / r.gqa) * (r.n_kv * r.gqa) + s.head * r.gqa +
-                                      f % r.gqa
-                                : -1,
+                f < s.n * r.gqa ? ((s.row0 + tok) * r.n_kv + s.head - tok) * r.gqa + f : -1,
                 0);  // (the tile's other rows' scores are not read)
       ca_take_q(S.q[buf], static_cast<const TQ*>(r.q), 0, a.negate);
       fence_proxy_async();
@@ -629,7 +622,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       CaSeg s{};
       if (left > 0) {
         int first, count;
-        ca_units(l.n, l.pos0, r.gqa, r.window, k, &first, &count);
+        ca_units(l.n, l.pos0, a.by_gqa, r.window, k, &first, &count);
         const int take = min(left, count - off);
         s = CaSeg{l.row0, l.n, l.pos0, k * kCaTile, lane, head, first + off, take, off == 0,
                   off + take == count};
@@ -660,7 +653,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       if (++seg_slot == kCaSegs) seg_slot = 0, seg_phase ^= 1;
       // its queries, wanted in a few microseconds, into L2
       const int lines = int(sizeof(TQ)) * r.gqa;  // of 128 bytes, per token and kv head
-      const int q0 = s.flat0 / r.gqa, q1 = min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
+      const int q0 = s.flat0 / a.by_gqa, q1 = min(s.n, (s.flat0 + kCaTile - 1) / a.by_gqa + 1);
       for (int e = wl; i > 0 && e < (q1 - q0) * lines; e += 32)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(
             static_cast<const char*>(r.q) +
@@ -680,13 +673,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     uint32_t phase = 0, tail_phase = 0;
     CaSeg s;
     while (ok && (ok = next_seg(&s)) && s.units > 0) {
-      const int last = min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
+      const int last = min(s.n, (s.flat0 + kCaTile - 1) / a.by_gqa + 1);
       const int hi = s.pos0 + last;  // positions from here on are seen by no row of the tile
       const int* table = r.block_table + (size_t)s.lane * r.max_blocks;
       const int end = min(hi, (s.unit0 + s.units) * kCaKeys);
       // this warp lane's box of the next unit: its position, block and (once read) page
       int p = s.unit0 * kCaKeys + wl * a.box;
-      const auto block = [&] { return a.odd ? 0 : int(__umulhi(p, a.div_m) >> a.div_s); };
+      const auto block = [&] { return a.odd ? 0 : p / a.by_page; };
       int blk = block(), page = wl < boxes && p < end ? table[blk] : -1;
       for (int j = 0; j < s.units; ++j) {
         const int p0 = (s.unit0 + j) * kCaKeys;
@@ -877,10 +870,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       w.f = s.flat0 + w.pr;
       w.live = w.f < s.n * r.gqa;
       w.work = __any_sync(0xffffffffu, w.live);
-      const int tok = w.f / r.gqa;
+      const int tok = w.f / a.by_gqa;
       w.pos = w.live ? s.pos0 + tok : -1;
       w.lo = r.window > 0 ? max(0, w.pos + 1 - r.window) : 0;
-      w.rh = w.live ? (s.row0 + tok) * (r.n_kv * r.gqa) + s.head * r.gqa + w.f % r.gqa : -1;
+      w.rh = w.live ? ((s.row0 + tok) * r.n_kv + s.head - tok) * r.gqa + w.f : -1;
       return w;
     };
     CaSeg s{};
@@ -1084,7 +1077,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           part[kCaTile * 129 + w.pr] = total;
         }
         unsigned again = __ballot_sync(0xffffffffu, w.live && probe != 0.f);
-        const int hi = s.pos0 + min(s.n, (s.flat0 + kCaTile - 1) / r.gqa + 1);
+        const int hi = s.pos0 + min(s.n, (s.flat0 + kCaTile - 1) / a.by_gqa + 1);
         while (again) {
           const int src = __ffs(again) - 1;
           again &= again - 1;
@@ -1161,6 +1154,7 @@ __global__ void __launch_bounds__(kCjThreads) chunk_attn_join_kernel(const CaArg
     }
   }
   if (f >= p.n * a.r.gqa) return;
+  const int tok = f / a.by_gqa;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint4 y[2];
   __half2* h = reinterpret_cast<__half2*>(y);
@@ -1170,8 +1164,8 @@ __global__ void __launch_bounds__(kCjThreads) chunk_attn_join_kernel(const CaArg
     h[2 * e + 1] = __floats2half2_rn(o[e].z * inv, o[e].w * inv);
   }
   uint4* dst = reinterpret_cast<uint4*>(
-      a.r.out + ((size_t)(p.row0 + f / a.r.gqa) * a.r.n_kv * a.r.gqa + p.head * a.r.gqa +
-                 f % a.r.gqa) * 128 + warp * 16);
+      a.r.out + ((size_t)((p.row0 + tok) * a.r.n_kv + p.head - tok) * a.r.gqa + f) * 128 +
+      warp * 16);
   dst[0] = y[0];
   dst[1] = y[1];
 }
@@ -1224,12 +1218,13 @@ cudaError_t launch_chunk_attn(const ChunkAttnRequest& r, int device, cudaStream_
   a.box = box;
   a.odd = odd;
   a.wide = (reinterpret_cast<uintptr_t>(r.out) & 31) == 0;
-  // for a divisor of 8 or more and dividends of 31 bits: m = floor(2^(31 + l) / d) + 1 with
-  // l = ceil(log2 d) is exact (Granlund and Montgomery 1994)
-  int l = 3;
-  while ((1ll << l) < r.block_size) ++l;
-  a.div_m = uint32_t((1ull << (31 + l)) / uint32_t(r.block_size) + 1);
-  a.div_s = l - 1;
+  const auto div = [](int d) {
+    int l = 0;
+    while ((1ll << l) < d) ++l;
+    return CaDiv{uint32_t((1ull << (31 + l)) / uint32_t(d) + 1), uint32_t(31 + l)};
+  };
+  a.by_page = div(r.block_size);
+  a.by_gqa = div(r.gqa);
   a.negate = r.scale < 0.f;
   // a scale of 0 still has to keep masked scores at -infinity
   a.c = fmaxf(fabsf(r.scale) * 1.4426950408889634f, 1e-30f);
