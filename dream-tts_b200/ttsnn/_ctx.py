@@ -24,7 +24,8 @@ def ctx(device: int | None = None) -> C.c_void_p:
 def ctx_of(t: torch.Tensor) -> C.c_void_p:
     if not t.is_cuda:
         raise ValueError("tts-nn (B200): tensors must live on a CUDA device; there is no CPU path")
-    return ctx(t.device.index)
+    dev = t.get_device()
+    return _ctx.get(dev) or ctx(dev)
 
 
 def stream() -> C.c_void_p:
@@ -33,12 +34,14 @@ def stream() -> C.c_void_p:
 
 def stream_of(t: torch.Tensor) -> int:
     """The current stream of the tensor's device (which need not be the current device)."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def as_type(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """t as contiguous `dtype` (a no-op `to` alone takes 2 us of a call's 10 on the host)."""
-    return (t if t.dtype == dtype else t.to(dtype)).contiguous()
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def ptr(t: torch.Tensor | None) -> C.c_void_p:

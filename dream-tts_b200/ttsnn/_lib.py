@@ -194,7 +194,7 @@ def load() -> C.CDLL:
 
 def call(name: str, *args) -> None:
     """Calls a tts_status-returning entry point and raises TtsError on failure."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != TTS_OK:
         msg = lib.tts_last_error()

@@ -106,10 +106,14 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
         raise ValueError("rotary: one contiguous int32 position per row")
     same_device("rotary", x, positions, cos, sin, out)
     c, s = _tables("rotary", cos, sin)
-    whole = lambda t: (t.stride(2) == 1 and t.stride(1) == hd and t.stride(0) % 8 == 0
-                       and t.stride(0) >= heads * hd and t.data_ptr() % 16 == 0)
+
+    def whole(t):
+        row, head, one = t.stride()
+        return (one == 1 and head == hd and row % 8 == 0 and row >= heads * hd
+                and t.data_ptr() % 16 == 0)
+
     if out is None:
-        y = torch.empty(rows, heads, hd, device=x.device, dtype=x.dtype)
+        y = x.new_empty((rows, heads, hd))
     else:
         if out.shape != x.shape or out.dtype != x.dtype or not whole(out):
             raise ValueError("rotary: out must have x's shape and type, heads side by side and "
@@ -118,9 +122,10 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
     if rows == 0:
         return y
     xc = x if whole(x) else x.contiguous()
-    L.call("tts_rotary", ctx_of(x), xc.data_ptr(), int(x.dtype == torch.float16), rows, heads, hd,
-           xc.stride(0), positions.data_ptr(), c.data_ptr(), s.data_ptr(), c.shape[0],
-           2 * c.shape[1], int(interleaved), y.data_ptr(), y.stride(0), stream_of(x))
+    length, pairs = c.shape
+    L.call("tts_rotary", ctx_of(x), xc.data_ptr(), x.dtype == torch.float16, rows, heads, hd,
+           xc.stride(0), positions.data_ptr(), c.data_ptr(), s.data_ptr(), length, 2 * pairs,
+           bool(interleaved), y.data_ptr(), y.stride(0), stream_of(x))
     return y
 
 
