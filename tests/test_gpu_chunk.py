@@ -178,6 +178,32 @@ def test_chunk_attention_runs_of_every_kind(tt, gqa, q32, seed):
     check_attention(tt, q.astype(np.float32 if q32 else np.float16), b)
 
 
+def test_chunk_attention_one_long_chunk(tt):
+    """More work tiles than a warp looks through at once, more lanes behind them."""
+    b = ck.batch(44, [1, 4300, 2, 500], [60, 70, 3, 0], 1, 16)
+    q = np.random.default_rng(45).standard_normal((int(b[0][-1]), 2, 128)).astype(np.float16)
+    check_attention(tt, q, b, window=150)
+
+
+def test_chunk_attention_shared_pages_and_unaligned_sectors(tt):
+    """Lanes over the same prefix pages; q and out on 16-byte, not 32-byte, boundaries."""
+    starts, spans, table, k, v = ck.batch(46, [40, 30, 1], [64, 64, 64], 2, 16)
+    table[1, :4] = table[2, :4] = table[0, :4]
+    q = np.random.default_rng(47).standard_normal((71, 4, 128)).astype(np.float16)
+    b = (starts, spans, table, k, v)
+    want = attend(tt, q, b)
+    mine = torch.empty(q.size + 8, device="cuda", dtype=torch.float16)
+    out = torch.empty(q.size + 16, device="cuda", dtype=torch.float16).fill_(3)
+    view, at = mine[8:].view(q.shape), out[8:-8].view(71, 512)
+    view.copy_(dev(q))
+    kv = tt.attn.paged_cache(dev(k), dev(v), dev(table))
+    tt.attn.chunk_attention(view, dev(starts), dev(spans), kv, SCALE, out=at)
+    tt.check()
+    assert torch.equal(at, want) and (out[:8] == 3).all() and (out[-8:] == 3).all()
+    exact, mass = ck.attention(q, *b, SCALE, 0, np.zeros((71, 512)))
+    assert (np.abs(host(want) - exact) <= ck.attention_bound(exact, mass)).all()
+
+
 def test_chunk_attention_pages_outside_pool(tt):
     b = ck.batch(11, [9, 40], [70, 30], 2, 16)
     starts, spans, table, k, v = b
