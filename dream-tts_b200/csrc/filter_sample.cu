@@ -18,13 +18,14 @@
 // of them are exact in 64 bits, so neither the order of the atomics nor the number of CTAs can
 // change a pick.
 //
-// Measured (192 rows of 151851 f32 ids, top-p 0.9): 243 us; reading them once takes 18. What bounds
+// Measured (192 rows of 151851 f32 ids, top-p 0.9): 233 us; reading them once takes 18. What bounds
 // it is the chain of a row's steps (load, maximum, bins, exchange, cut, draw), each behind a
-// barrier of the CTA or cluster: issue slots are 41 % used, a row alone takes 31 us, and some 36
+// barrier of the CTA or cluster: issue slots are 41 % used, a row alone takes 30 us, and some 36
 // rows are at work at a time. So the row stays in shared memory, two CTAs share an SM, and CTAs
-// exchange little. (The bins cost 61 us of it in atomics and 47 besides; 512 of them 276 us, 2048
-// 247. Clusters of 16 CTAs 399 to 461.) 48 rows of 32003 with every filter 23 us, 8 rows of 2048
-// with top-k alone 10 us.
+// exchange little. (The bins cost 61 us of it in atomics, 32 bits at a time: 64 at once, 319 us;
+// of 247 us then, 512 bins took 276, 2048 took 247, clusters of 16 CTAs 399 to 461.) 48 rows of
+// 32003 with every filter 22 us, 8 rows of 2048 with top-k alone 10 us.
+#include <cfloat>
 #include <mutex>
 
 #include "tts_common.cuh"
@@ -40,8 +41,9 @@ constexpr int kFsWarps = kFsThreads / 32;
 constexpr int kFsBins = 1024;
 constexpr int kFsLoads = 4;      // 16-byte loads a thread has on their way
 constexpr int kFsCap = 1024;     // ids the first CTA sorts at once
-// ... without cutting the list into parts first (192 rows of 151851: 247 us, all sorted whole 287)
-constexpr int kFsFew = 96;
+// ... without cutting the list into parts first (512 rows of 32000: 121 us, 125 where only 96 are;
+// 192 rows of 151851, lists of 600: 247 us, 287 where all are)
+constexpr int kFsFew = 256;
 constexpr int kFsMaxCluster = 8;
 constexpr float kFsOctaves = 45.f;  // below 2^-45 a weight is 0
 // Ids in a CTA's part up to which two CTAs share an SM (192 rows of 151851: two 247 us, one with
@@ -79,6 +81,7 @@ struct FsSmem {
   u64 share[2][kFsMaxCluster];  // one value of each CTA, two uses in turn
   u64 answer;                   // what one thread, or the first CTA, found
   uint32_t mine;                // ids this CTA gathers
+  int found;                    // by fs_reach
   int digit_at;                 // the part of the keys that a target falls into
   u64 digit_below[2];           // and the weight and count above it
   alignas(16) float x[4];       // this CTA's part of the row (a.per entries), -inf: never picked
@@ -173,9 +176,13 @@ TTS_DEV u64 fs_before(FsSmem& S, u64 v) {
 // The first place at which a running sum (inclusive, `n` entries) reaches `target`: `n` if none.
 template <typename F>
 TTS_DEV int fs_reach(FsSmem& S, int n, u64 target, F sum_at) {
-  u64 below = 0;
-  for (int i = threadIdx.x; i < n; i += kFsThreads) below += sum_at(i) < target;
-  return int(fs_sum(S, below));
+  __syncthreads();
+  if (threadIdx.x == 0) S.found = n;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kFsThreads)
+    if (sum_at(i) >= target && (i == 0 || sum_at(i - 1) < target)) S.found = i;
+  __syncthreads();
+  return S.found;
 }
 
 // The sums of the row's CTAs, in all of them: each adds up a share of the entries.
@@ -230,6 +237,23 @@ TTS_DEV void fs_each(const FsSmem& S, int n, F f) {
   }
 }
 
+// f(i, x) for those of them from low to high (both finite or low below all), where they are few.
+template <typename F>
+TTS_DEV void fs_each_in(const FsSmem& S, int n, float low, float high, F f) {
+  low = fmaxf(low, -FLT_MAX);  // not the padding, nor what may not be picked
+#pragma unroll 2
+  for (int i = threadIdx.x * 4; i < n; i += kFsThreads * 4) {
+    const float4 v = *reinterpret_cast<const float4*>(S.x + i);
+    const bool x = v.x >= low && v.x <= high, y = v.y >= low && v.y <= high,
+               z = v.z >= low && v.z <= high, w = v.w >= low && v.w <= high;
+    if (!(x || y || z || w)) continue;
+    if (x) f(i, v.x);
+    if (y) f(i + 1, v.y);
+    if (z) f(i + 2, v.z);
+    if (w) f(i + 3, v.w);
+  }
+}
+
 // Counts the row's ids of the given bins and keys and, if the first CTA's list holds them all, puts
 // them there, each CTA's behind those of the CTAs before it.
 TTS_DEV int fs_gather(FsSmem& S, const FsScale& r, int n, int id0, uint32_t rank, uint32_t ctas,
@@ -240,8 +264,7 @@ TTS_DEV int fs_gather(FsSmem& S, const FsScale& r, int n, int id0, uint32_t rank
   __syncthreads();
   if (t == 0) S.mine = 0;
   __syncthreads();
-  fs_each(S, n, [&](int i, float x) {
-    if (x < low || x > high) return;
+  fs_each_in(S, n, low, high, [&](int i, float x) {
     const int b = r.bin(x);
     const uint32_t k = float_order_key(x);
     if (b < bin0 || b > bin1 || k < key0 || k > key1) return;
