@@ -136,6 +136,18 @@ def test_chunk_attention_scales(tt, scale):
     assert (np.abs(got - want) <= ck.attention_bound(want, mass) + slack).all()
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.7])
+def test_chunk_attention_scales_of_f32_queries(tt, scale):
+    b = ck.batch(36, [33, 1, 150, 2, 1, 1], [200, 150, 0, 7, 300, 1], 2, 16)
+    q = np.random.default_rng(37).standard_normal((188, 4, 128)).astype(np.float32)
+    got = host(attend(tt, q, b, scale=scale))
+    want, mass = ck.attention(q, *b, scale, 0, np.zeros((188, 512)))
+    # f32 scores of up to ~30: their rounding (2^-24 each of 128 products and sums) adds to the bound,
+    # and so does what two f16 pieces leave of a query (2^-22 of it)
+    slack = (2.0 ** -24 * 128 + 2.0 ** -22) * 40 * abs(scale) * mass
+    assert (np.abs(got - want) <= ck.attention_bound(want, mass) + slack).all()
+
+
 def test_chunk_attention_two_streams_at_once(tt):
     """Calls that overlap on the GPU have a workspace each."""
     args = []
