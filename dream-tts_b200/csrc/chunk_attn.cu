@@ -9,7 +9,7 @@
 // (two MMAs a query tile and unit: S = Q.K^T, O += P.V). While one query tile's softmax runs, the
 // tensor cores work on the other. Where there is one query tile only (a token or a few), its units
 // alternate between the two score buffers and groups of softmax warps, each with an O of its own,
-// and the first group reads both at the end (48 single rows over 4300 positions: 148 us; as two
+// and the first group reads both at the end (48 single rows over 4300 positions: 150 us; as two
 // query tiles, one of them empty, 182).
 //
 // Split. The units of all work tiles, one after another, are cut into equal runs, one per SM; a
@@ -27,14 +27,14 @@
 // for it after the first units), so no maximum is looked for in most units. Weights keep f16's 11
 // bits down to 2^-22 of r's; sums are f32.
 //
-// Measured (16 q heads, 8 kv heads): 4096 new rows over 12288 positions 435 us, 1106 TFLOP/s, 64 %
+// Measured (16 q heads, 8 kv heads): 4096 new rows over 12288 positions 430 us, 1118 TFLOP/s, 65 %
 // of a large plain product's rate: a unit of two query tiles takes about 3.9k clocks, its MMAs 2.4k
 // to 2.9k and its exponentials 2.0k (16 a clock) of them, the rest is their hand-overs. With f32
-// queries 553 us: the scores are two products. 48 single rows over 4300 positions 148 us, 5.7 TB/s,
-// 88 % of a copy: bound by HBM. 448 single rows over 300: 184 us, 3.0 TB/s, and 592 chunks of 128
-// rows 41 us: runs of one to three units are too short to hide their start and end (about 10k
-// clocks). There the fetch of instructions counts, so loops over a unit stay rolled and queries
-// come by copies in short loops: unrolled, those two took 325 and 54 us.
+// queries 553 us: the scores are two products. 48 single rows over 4300 positions 146 us, 5.8 TB/s,
+// 90 % of a copy: bound by HBM. 448 single rows over 300: 180 us, 3.1 TB/s, and 592 chunks of 128
+// rows 40 us: runs of one to three units are too short to hide their start and end (about 10k
+// clocks). There the fetch of instructions counts, so loops over a unit stay rolled, queries come
+// by copies in short loops and divisions are multiplications: unrolled, those two took 325 and 54.
 #include <mutex>
 
 #include "chunk_batch.cuh"
@@ -161,8 +161,8 @@ struct Int {
 // A run of no more rows than a warp loads at once: its queries are loaded by the warp that walks
 // the work, into the other buffer than the run before's if that was one too, while that is at work.
 // Any other run's are loaded by the softmax warps, tile tl's into buffer tl, when the run before is
-// done (a warp takes about a microsecond for 32 rows: chunks of 512 rows 149 us with all queries
-// loaded by the one, 106 this way).
+// done (a warp takes about a microsecond for 32 rows: 16 chunks of 512 rows over 512 took 149 us
+// with all queries loaded by the one, 106 this way).
 TTS_DEV bool ca_few(const CaSeg& s, int gqa) { return s.n * gqa - s.flat0 <= 32; }
 TTS_DEV int ca_q_buffer(bool few, bool last_few, int last) {
   return few && last_few ? last ^ 1 : 0;
