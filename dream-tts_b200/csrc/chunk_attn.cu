@@ -35,6 +35,7 @@
 // rows 40 us: runs of one to three units are too short to hide their start and end (about 10k
 // clocks). There the fetch of instructions counts, so loops over a unit stay rolled, queries come
 // by copies in short loops and divisions are multiplications: unrolled, those two took 325 and 54.
+#include <cfloat>
 #include <mutex>
 
 #include "chunk_batch.cuh"
@@ -74,8 +75,12 @@ TTS_DEV uint32_t ca_sign(uint32_t two_halves, int negate) {
 // The warp's 32 query rows (`rh`: each lane's row of q [rows * heads][128], -1: zeros) on their way
 // to rows r0 .. r0 + 31 of the tile (copies in a short loop: unrolled loads to registers took
 // longer to fetch their instructions than to arrive), and what is to be done once they are there.
-// Half a warp takes a row of f16, a warp a row of f32, which is split into two f16 pieces (22 bits)
-// so that the scores keep f32 queries' precision.
+// Half a warp takes a row of f16, a warp a row of f32, which is split into two f16 pieces so that
+// the scores keep f32 queries' precision. Before that the row is multiplied by a power of two that
+// brings its largest magnitude to [2^14, 2^15), just inside f16's range; its softmax factor is
+// divided by it (ca_factor). So the pieces hold 22 bits of an element, or 2^-39 of the row's
+// largest where that is more, whatever the row's magnitude (unscaled, elements past 65504 were
+// infinite and a row near 1e-5 lost 1e-3 of its result).
 TTS_DEV void ca_copy_q(uint8_t (*tile)[kCaTileBytes], const __half* q, int rh, int r0) {
   const int wl = threadIdx.x & 31, sub = wl >> 4, e = wl & 15;
 #pragma unroll 2
@@ -84,7 +89,7 @@ TTS_DEV void ca_copy_q(uint8_t (*tile)[kCaTileBytes], const __half* q, int rh, i
     ca_copy(&tile[0][ca_at(r0 + 2 * k + sub, e)], q + (size_t)max(at, 0) * 128 + e * 8, at >= 0);
   }
 }
-TTS_DEV void ca_take_q(uint8_t (*tile)[kCaTileBytes], const __half*, int r0, int negate) {
+TTS_DEV void ca_take_q(uint8_t (*tile)[kCaTileBytes], const __half*, int r0, int negate, uint8_t*) {
   const int wl = threadIdx.x & 31, sub = wl >> 4, e = wl & 15;
   ca_copy_wait();
   if (!negate) return;
@@ -103,8 +108,22 @@ TTS_DEV void ca_copy_q(uint8_t (*tile)[kCaTileBytes], const float* q, int rh, in
     ca_copy(&tile[wl & 1][ca_at(r0 + k, wl >> 1)], q + (size_t)max(at, 0) * 128 + wl * 4, at >= 0);
   }
 }
-TTS_DEV void ca_take_q(uint8_t (*tile)[kCaTileBytes], const float*, int r0, int negate) {
+// The exponent (biased) of a row whose largest magnitude has these bits, what the row is multiplied
+// by and what its scores' factor is then; rows below 2^-112 are scaled like those at it (f32 has no
+// finer element there than the pieces hold), infinities and NaN stay what they are.
+TTS_DEV uint32_t ca_exponent(uint32_t largest) { return max(largest >> 23, 15u); }
+TTS_DEV float ca_scale_up(uint32_t exponent) { return __uint_as_float((268u - exponent) << 23); }
+// Factors are kept above 0 (times -infinity) and far below infinity: scores are multiples of 2^-48
+// and below 2^39, so a factor of 2^80 parts any two of them as a larger one would.
+constexpr float kCaFlat = 1e-30f, kCaSteep = 1.2089258196146292e24f;  // 2^80
+TTS_DEV float ca_factor(float c, uint32_t exponent) {
+  return fminf(fmaxf(c * __uint_as_float((exponent - 14u) << 23), kCaFlat), kCaSteep);
+}
+// Leaves the rows' exponents in `exponents` (null: rows of nothing).
+TTS_DEV void ca_take_q(uint8_t (*tile)[kCaTileBytes], const float*, int r0, int negate,
+                       uint8_t* exponents) {
   const int wl = threadIdx.x & 31;
+  uint32_t mine = 0;
   ca_copy_wait();
 #pragma unroll 1
   for (int k0 = 0; k0 < 32; k0 += 4) {
@@ -115,6 +134,12 @@ TTS_DEV void ca_take_q(uint8_t (*tile)[kCaTileBytes], const float*, int r0, int 
     __syncwarp();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+      const float most =
+          fmaxf(fmaxf(fabsf(x[k].x), fabsf(x[k].y)), fmaxf(fabsf(x[k].z), fabsf(x[k].w)));
+      const uint32_t e = ca_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+      if (wl == k0 + k) mine = e;
+      const float up = ca_scale_up(e);
+      x[k] = make_float4(x[k].x * up, x[k].y * up, x[k].z * up, x[k].w * up);
       const __half2 h0 = __floats2half2_rn(x[k].x, x[k].y), h1 = __floats2half2_rn(x[k].z, x[k].w);
       const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
       const __half2 l0 = __floats2half2_rn(x[k].x - b0.x, x[k].y - b0.y),
@@ -128,6 +153,7 @@ TTS_DEV void ca_take_q(uint8_t (*tile)[kCaTileBytes], const float*, int r0, int 
                      ca_sign(*reinterpret_cast<const uint32_t*>(&l1), negate));
     }
   }
+  if (exponents) exponents[wl] = uint8_t(mine);
 }
 
 // One run of a work tile's units.
@@ -150,6 +176,10 @@ struct CaSmem {
   int start[4];  // the CTA's first lane, work tile, head and unit
   int count;     // its units
   int4 box_row[2][kCaKeys / 32];  // the loaders' boxes: their pool rows, -1 where none is read
+  // f32 queries' exponents: of tiles that the softmax warps load, by tile (read by the warps that
+  // wrote them or, of a lone tile, after they have met), of few rows by run (a run's place is
+  // written again four runs later, when all warps have left it)
+  uint8_t q_exp[kParts - 1 ? 2 : 1][128], few_exp[kCaSegs][32];
   uint32_t tmem;
 };
 
@@ -191,7 +221,7 @@ TTS_DEV int operator/(int n, CaDiv d) { return int((uint64_t(uint32_t(n)) * d.m)
 
 struct CaArgs {
   ChunkAttnRequest r;
-  float c;      // |scale| log2 e
+  float c;      // |scale| log2 e; f32 queries' rows have their own (ca_factor)
   int negate;   // scale < 0: the queries change sign
   int box;      // rows of a page that one copy takes
   int odd;      // one page per lane, of no multiple of 8 rows
@@ -395,8 +425,8 @@ TTS_DEV long ca_pool_row(const CaArgs& a, int lane, int head, int pos) {
 // held beyond what it sees and, if one is not finite, sums the row again over what it sees (dims
 // 4 lane .. + 3 of the result to each warp lane). Never reached by finite caches.
 template <typename TQ>
-__device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, int hi, float ref,
-                                       float4* o) {
+__device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, int hi, float c,
+                                       float ref, float4* o) {
   const int wl = threadIdx.x & 31;
   const int tok = f / a.by_gqa, head = s.head * a.r.gqa + f - tok * a.r.gqa;
   const int pos = s.pos0 + tok;
@@ -417,6 +447,13 @@ __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, i
   float q[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) q[i] = ca_q<TQ>(a, s.row0 + tok, head, wl * 4 + i);
+  if (sizeof(TQ) == 4) {  // as the scores' queries were
+    const float most = fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3])));
+    const float up =
+        ca_scale_up(ca_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(most))));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] *= up;
+  }
   *o = make_float4(0.f, 0.f, 0.f, 0.f);
   const float bias = ref == -INFINITY ? 0.f : kCaBias - ref;
   for (int p = max(u0, lo); p < min(u1, pos + 1); ++p) {
@@ -426,7 +463,7 @@ __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, i
     const __half2* v = reinterpret_cast<const __half2*>(a.r.v_pool + at * 128 + wl * 4);
     const float2 k0 = __half22float2(k[0]), k1 = __half22float2(k[1]);
     const float x = warp_sum(q[0] * k0.x + q[1] * k0.y + q[2] * k1.x + q[3] * k1.y);
-    const float w = ex2(fmaf(x, a.c, bias));
+    const float w = ex2(fmaf(x, c, bias));
     const float2 v0 = __half22float2(v[0]), v1 = __half22float2(v[1]);
     o->x += w * v0.x, o->y += w * v0.y, o->z += w * v1.x, o->w += w * v1.y;
   }
@@ -612,7 +649,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       ca_copy_q(S.q[buf], static_cast<const TQ*>(r.q),
                 f < s.n * r.gqa ? ((s.row0 + tok) * r.n_kv + s.head - tok) * r.gqa + f : -1,
                 0);  // (the tile's other rows' scores are not read)
-      ca_take_q(S.q[buf], static_cast<const TQ*>(r.q), 0, a.negate);
+      ca_take_q(S.q[buf], static_cast<const TQ*>(r.q), 0, a.negate, S.few_exp[i % kCaSegs]);
       fence_proxy_async();
       __syncwarp();
       if (wl < 4) mbar_arrive(&S.q_full[buf]);
@@ -884,6 +921,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       const int lo_max = __reduce_max_sync(0xffffffffu, w.live ? w.lo : 0);
       float ref = w.live ? -INFINITY : 0.f, sum = 0.f;
       bool fresh = true;  // some row has no reference yet
+      float c = a.c;      // of scores as they come from the MMAs
       const int step0 = w.one ? tl : 0, steps = w.one ? 2 : 1;
       for (int j = step0; j < s.units; j += steps) {
         ok = ca_wait(&S.s_full[tl], s_phase);
@@ -894,6 +932,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           const int p0 = (s.unit0 + j) * kCaKeys;
           const bool edge = p0 + kCaKeys - 1 > pos_min || p0 < lo_max;
           const int first = w.lo - p0, last = w.pos - p0;  // columns the row sees
+          if (kParts > 1 && j == step0)
+            c = ca_factor(a.c, w.few ? S.few_exp[(seg_slot + kCaSegs - 1) % kCaSegs][wl]
+                                     : S.q_exp[(w.one ? 0 : tl) & (kParts - 1)][lane_row]);
           // the unit's positions in two halves: their scores in x, their weights over them in TMEM
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
@@ -921,7 +962,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 // O holds weights against the old reference: bring it, and the sum, to the new one
                 float up = ref;
                 if (raise) {
-                  up = ca_max<kCaHalf>(x, a.c, ref);
+                  up = ca_max<kCaHalf>(x, c, ref);
                   if (up == INFINITY) up = NAN;  // as the row's formula has it
                 }
                 const float keep = up == -INFINITY ? 1.f : ex2(ref - up);
@@ -946,7 +987,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 }
               }
               uint32_t y[kCaHalf / 2];
-              got = ca_weights<kCaHalf>(x, y, a.c, ref);
+              got = ca_weights<kCaHalf>(x, y, c, ref);
               tmem_st16(s_at + c0 / 2, y);
               tmem_st16(s_at + c0 / 2 + 16, y + 16);
               raise = !(got <= kCaMost) && ref == ref;
@@ -1013,7 +1054,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       }
       if (load) {
         if (w.one) ca_copy_q(S.q[tl], static_cast<const TQ*>(r.q), wn.rh, (warp & 3) * 32);
-        ca_take_q(S.q[tl], static_cast<const TQ*>(r.q), (warp & 3) * 32, a.negate);
+        // (few rows here: the first run's)
+        uint8_t* const exponents = kParts == 1 ? nullptr
+                                   : !wn.few   ? &S.q_exp[tl & (kParts - 1)][(warp & 3) * 32]
+                                   : warp == 0 ? S.few_exp[0]
+                                               : nullptr;
+        ca_take_q(S.q[tl], static_cast<const TQ*>(r.q), (warp & 3) * 32, a.negate, exponents);
         fence_proxy_async();
         tc_fence_before();
         __syncwarp();
@@ -1082,12 +1128,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           const int src = __ffs(again) - 1;
           again &= again - 1;
           float4 y;
+          const float sc = __shfl_sync(0xffffffffu, c, src);
           const float sref = __shfl_sync(0xffffffffu, ref, src);
           const float sinv = __shfl_sync(0xffffffffu, inv, src);
           const int sf = __shfl_sync(0xffffffffu, w.f, src);
           const int spr = __shfl_sync(0xffffffffu, w.pr, src);
           const int at = __shfl_sync(0xffffffffu, w.rh, src);
-          if (!ca_repair<TQ>(a, s, sf, hi, sref, &y)) continue;
+          if (!ca_repair<TQ>(a, s, sf, hi, sc, sref, &y)) continue;
           __syncwarp();  // after the row's own stores
           if (whole) {
             __half2* h = reinterpret_cast<__half2*>(r.out + (size_t)at * 128 + wl * 4);
@@ -1226,8 +1273,10 @@ cudaError_t launch_chunk_attn(const ChunkAttnRequest& r, int device, cudaStream_
   a.by_page = div(r.block_size);
   a.by_gqa = div(r.gqa);
   a.negate = r.scale < 0.f;
-  // a scale of 0 still has to keep masked scores at -infinity
-  a.c = fmaxf(fabsf(r.scale) * 1.4426950408889634f, 1e-30f);
+  // f32 queries: kept in range row by row (ca_factor); f16: here
+  const double c = fabs(double(r.scale)) * 1.4426950408889634;
+  a.c = r.q_f16 ? float(fmin(fmax(c, double(kCaFlat)), double(kCaSteep)))
+                : float(fmin(c, double(FLT_MAX)));
   a.parts = static_cast<CaPart*>(r.workspace);
   a.part_data = reinterpret_cast<float*>(a.parts + 2 * ctas);
   cudaError_t e = r.q_f16 ? launch_as<__half, 3, 2, 1>(tmK, tmV, a, ctas, device, st)

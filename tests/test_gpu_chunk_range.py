@@ -1,0 +1,99 @@
+"""Chunk attention over the whole range of its arguments: magnitudes of f32 queries, scales."""
+import numpy as np
+import pytest
+import torch
+
+import _chunks as ck
+
+pytestmark = pytest.mark.gpu
+SCALE = 128 ** -0.5
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def attend(tt, q, b, scale=SCALE, window=0, out=None):
+    starts, spans, table, k, v = b
+    kv = tt.attn.paged_cache(dev(k), dev(v), dev(table))
+    o = tt.attn.chunk_attention(dev(q), dev(starts), dev(spans), kv, scale, window, out)
+    return o.cpu().numpy().astype(np.float64)
+
+
+def score_error(q, b, scale):
+    """What f32 scores may be off by: of the largest sum of |scale q_d k_d| of a row and a position
+    128 products and sums of half a step each and 2^-22 of what two f16 pieces leave of a query's
+    element, 2^-39 of its row's largest where that is more."""
+    starts, spans, table, k, v = b
+    n_kv, most = k.shape[1], 0.0
+    gqa = q.shape[1] // n_kv
+    for i in range(len(spans)):
+        kc = np.abs(ck.lane_rows(k, table, i, int(spans[i])))
+        rows = np.abs(q[starts[i]:starts[i + 1]].astype(np.float64)).reshape(-1, n_kv, gqa, 128)
+        for h in range(n_kv if len(kc) and len(rows) else 0):
+            most = max(most, (rows[:, h] @ kc[:, h].T).max() * (128 * 2.0 ** -24 + 2.0 ** -22)
+                       + 2.0 ** -39 * (rows[:, h].max(-1)[..., None] * kc[:, h].sum(-1)).max())
+    return most * abs(scale)
+
+
+def within(q, b, got, scale):
+    """attention_bound, and twice (weights and their sum) what the scores may be off by."""
+    want, mass = ck.attention(q, *b, scale, 0, np.zeros(got.shape))
+    slack = 2 * score_error(q, b, scale) * mass
+    off = np.abs(got - want) - ck.attention_bound(want, mass) - slack
+    assert not np.isnan(got).any() and off.max() <= 0, (off.max(), np.argwhere(off > 0)[:4])
+
+
+@pytest.mark.parametrize("size", [1e-38, 1e-30, 1e-7, 1e-5, 1e-3, 30.0, 1e5, 1e9, 1e37])
+def test_f32_queries_of_any_size(tt, size):
+    """The same scores from queries of any magnitude, `scale` making up for it."""
+    b = ck.batch(61, [1, 40, 150, 3, 2, 70, 1], [200, 30, 0, 129, 7, 300, 400], 2, 16)
+    q = (np.random.default_rng(62).standard_normal((int(b[0][-1]), 4, 128)) * size).astype(np.float32)
+    scale = float(np.float32(SCALE / size))
+    within(q, b, attend(tt, q, b, scale), scale)
+    tt.check()
+
+
+@pytest.mark.parametrize("gqa,seed", [(2, 63), (8, 64)])
+def test_f32_queries_of_a_size_for_each_row(tt, gqa, seed):
+    """Rows of very different magnitudes beside one another, in runs of every kind."""
+    rng = np.random.default_rng(seed)
+    new = rng.choice([1, 1, 2, 4, 5, 15, 17, 33, 64, 70, 129, 0], 300)
+    b = ck.batch(seed, new, rng.choice([0, 0, 3, 60, 130, 300], 300), 2, 16)
+    q = rng.standard_normal((int(b[0][-1]), 2 * gqa, 128))
+    q *= rng.choice([1e-20, 1e-6, 0.01, 0.3, 1, 3], (q.shape[0], q.shape[1], 1))
+    q = q.astype(np.float32)
+    within(q, b, attend(tt, q, b), SCALE)
+    tt.check()
+
+
+def test_f32_queries_of_a_size_for_each_dim(tt):
+    """Dims a million times smaller than their row's largest, beside keys as much larger."""
+    starts, spans, table, k, v = ck.batch(65, [40, 1], [200, 300], 2, 16)
+    small = np.arange(128) % 2 == 1
+    k[..., ~small] *= 2.0 ** -10
+    k[..., small] *= 2.0 ** 10
+    q = np.random.default_rng(66).standard_normal((41, 4, 128))
+    q[..., ~small] *= 2.0 ** 10
+    q[..., small] *= 2.0 ** -10
+    b = (starts, spans, table, k, v)
+    q = q.astype(np.float32)
+    within(q, b, attend(tt, q, b), SCALE)
+
+
+def test_f32_queries_of_zero_infinity_and_nan(tt):
+    """Rows of zeros weigh all positions alike; a row with an infinity or NaN is NaN, alone."""
+    b = ck.batch(69, [60, 1, 2], [30, 100, 3], 2, 16)
+    q = np.random.default_rng(70).standard_normal((63, 4, 128)).astype(np.float32)
+    q[[3, 60], :] = 0
+    q[5, 1, 7] = np.nan
+    q[40, 2, 100] = np.inf
+    got = attend(tt, q, b).reshape(63, 4, 128)
+    assert np.isnan(got[5, 1]).all() and np.isnan(got[40, 2]).all()
+    q[5, 1], q[40, 2], got[5, 1], got[40, 2] = 0, 0, 0, 0
+    want, mass = ck.attention(q, *b, SCALE, 0, np.zeros((63, 512)))
+    want, mass = want.reshape(63, 4, 128), mass.reshape(63, 4, 128)
+    want[5, 1], want[40, 2] = 0, 0
+    slack = 2 * score_error(q, b, SCALE) * mass
+    assert (np.abs(got - want) <= ck.attention_bound(want, mass) + slack).all()
+    tt.check()
