@@ -277,10 +277,20 @@ TTS_DEV float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return y;
 }
-// The f16 weights of N scores (-inf: not seen) against `ref`, two to a word, and their sum.
+// A row's weights are 2^(c s + bias). Past |ref| = 2^22 both are smaller by a power of two: c s is
+// rounded by half a step of itself, beyond 2^27 by more than the weights' room of 2^8, and scores
+// that the slope of 2^22 does not part differ by less than f32 sums of 128 products resolve.
+struct CaAim {
+  float c, bias;
+};
+TTS_DEV CaAim ca_aim(float c, float ref) {
+  const uint32_t e = __float_as_uint(ref) >> 23 & 255u;
+  const float less = __uint_as_float((127u - (e > 149u ? e - 149u : 0u)) << 23);
+  return ref == -INFINITY ? CaAim{c, 0.f} : CaAim{c * less, kCaBias - ref * less};
+}
+// The f16 weights of N scores (-inf: not seen), two to a word, and their sum.
 template <int N>
-TTS_DEV float ca_weights(const uint32_t* v, uint32_t* y, float c, float ref) {
-  const float bias = ref == -INFINITY ? 0.f : kCaBias - ref;
+TTS_DEV float ca_weights(const uint32_t* v, uint32_t* y, float c, float bias) {
   const float2 c2 = make_float2(c, c), b2 = make_float2(bias, bias);
   // batches of 4 pairs, the exponentials of the next on their way while one is summed and packed
   float2 w[2][4], part[4];
@@ -425,8 +435,8 @@ TTS_DEV long ca_pool_row(const CaArgs& a, int lane, int head, int pos) {
 // held beyond what it sees and, if one is not finite, sums the row again over what it sees (dims
 // 4 lane .. + 3 of the result to each warp lane). Never reached by finite caches.
 template <typename TQ>
-__device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, int hi, float c,
-                                       float ref, float4* o) {
+__device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, int hi, CaAim aim,
+                                       float4* o) {
   const int wl = threadIdx.x & 31;
   const int tok = f / a.by_gqa, head = s.head * a.r.gqa + f - tok * a.r.gqa;
   const int pos = s.pos0 + tok;
@@ -455,7 +465,6 @@ __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, i
     for (int i = 0; i < 4; ++i) q[i] *= up;
   }
   *o = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float bias = ref == -INFINITY ? 0.f : kCaBias - ref;
   for (int p = max(u0, lo); p < min(u1, pos + 1); ++p) {
     const long at = ca_pool_row(a, s.lane, s.head, p);
     if (at < 0) continue;
@@ -463,7 +472,7 @@ __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, i
     const __half2* v = reinterpret_cast<const __half2*>(a.r.v_pool + at * 128 + wl * 4);
     const float2 k0 = __half22float2(k[0]), k1 = __half22float2(k[1]);
     const float x = warp_sum(q[0] * k0.x + q[1] * k0.y + q[2] * k1.x + q[3] * k1.y);
-    const float w = ex2(fmaf(x, c, bias));
+    const float w = ex2(fmaf(x, aim.c, aim.bias));
     const float2 v0 = __half22float2(v[0]), v1 = __half22float2(v[1]);
     o->x += w * v0.x, o->y += w * v0.y, o->z += w * v1.x, o->w += w * v1.y;
   }
@@ -920,6 +929,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       const int pos_min = __reduce_min_sync(0xffffffffu, w.live ? w.pos : INT_MAX);
       const int lo_max = __reduce_max_sync(0xffffffffu, w.live ? w.lo : 0);
       float ref = w.live ? -INFINITY : 0.f, sum = 0.f;
+      CaAim aim;
       bool fresh = true;  // some row has no reference yet
       float c = a.c;      // of scores as they come from the MMAs
       const int step0 = w.one ? tl : 0, steps = w.one ? 2 : 1;
@@ -935,6 +945,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           if (kParts > 1 && j == step0)
             c = ca_factor(a.c, w.few ? S.few_exp[(seg_slot + kCaSegs - 1) % kCaSegs][wl]
                                      : S.q_exp[(w.one ? 0 : tl) & (kParts - 1)][lane_row]);
+          if (j == step0) aim = ca_aim(c, ref);
           // the unit's positions in two halves: their scores in x, their weights over them in TMEM
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
@@ -967,6 +978,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 }
                 const float keep = up == -INFINITY ? 1.f : ex2(ref - up);
                 ref = up;
+                aim = ca_aim(c, ref);
                 sum *= keep;
                 fresh = __any_sync(0xffffffffu, ref == -INFINITY);
                 if (h > 0) {  // the first half's MMAs; before that, S(j) came after all others
@@ -987,7 +999,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 }
               }
               uint32_t y[kCaHalf / 2];
-              got = ca_weights<kCaHalf>(x, y, c, ref);
+              got = ca_weights<kCaHalf>(x, y, aim.c, aim.bias);
               tmem_st16(s_at + c0 / 2, y);
               tmem_st16(s_at + c0 / 2 + 16, y + 16);
               raise = !(got <= kCaMost) && ref == ref;
@@ -1128,13 +1140,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           const int src = __ffs(again) - 1;
           again &= again - 1;
           float4 y;
-          const float sc = __shfl_sync(0xffffffffu, c, src);
-          const float sref = __shfl_sync(0xffffffffu, ref, src);
+          const CaAim own = ca_aim(c, ref);
+          const CaAim saim{__shfl_sync(0xffffffffu, own.c, src),
+                           __shfl_sync(0xffffffffu, own.bias, src)};
           const float sinv = __shfl_sync(0xffffffffu, inv, src);
           const int sf = __shfl_sync(0xffffffffu, w.f, src);
           const int spr = __shfl_sync(0xffffffffu, w.pr, src);
           const int at = __shfl_sync(0xffffffffu, w.rh, src);
-          if (!ca_repair<TQ>(a, s, sf, hi, sc, sref, &y)) continue;
+          if (!ca_repair<TQ>(a, s, sf, hi, saim, &y)) continue;
           __syncwarp();  // after the row's own stores
           if (whole) {
             __half2* h = reinterpret_cast<__half2*>(r.out + (size_t)at * 128 + wl * 4);

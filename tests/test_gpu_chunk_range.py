@@ -97,3 +97,61 @@ def test_f32_queries_of_zero_infinity_and_nan(tt):
     slack = 2 * score_error(q, b, SCALE) * mass
     assert (np.abs(got - want) <= ck.attention_bound(want, mass) + slack).all()
     tt.check()
+
+
+@pytest.mark.parametrize("q32,size,scale", [(False, 1, 2e38), (True, 1, 2e38), (True, 1e38, 2e38),
+                                            (True, 1e38, 1.0), (False, 1, 1e30), (True, 1, -2e38),
+                                            (False, 1, 1e9), (True, 1, 3e10), (True, 1e5, 7e6),
+                                            (False, 1, -1e12), (True, 1e9, 1.3)])
+def test_scores_past_f32(tt, q32, size, scale):
+    """Scores far apart, past f32's range: the largest takes it all. Rows whose two largest scores
+    are nearer than f32 sums tell apart are left out; a few queries of 1e38 are infinite as f32, their
+    rows NaN."""
+    b = ck.batch(67, [30, 1, 2], [60, 200, 3], 2, 16)
+    q = (np.random.default_rng(68).standard_normal((33, 4, 128)) * size)
+    with np.errstate(over="ignore"):
+        q = q.astype(np.float32 if q32 else np.float16)
+    got = attend(tt, q, b, scale)
+    starts, spans, table, k, v = b
+    told = 0
+    for i in range(3):
+        kc, vc = ck.lane_rows(k, table, i, int(spans[i])), ck.lane_rows(v, table, i, int(spans[i]))
+        for j in range(starts[i + 1] - starts[i]):
+            p = spans[i] - (starts[i + 1] - starts[i]) + j
+            for h in range(4):
+                if not np.isfinite(q[starts[i] + j, h]).all():
+                    assert np.isnan(got[starts[i] + j, h * 128:h * 128 + 128]).all()
+                    continue
+                s = kc[:p + 1, h // 2] @ q[starts[i] + j, h].astype(np.float64) * np.sign(scale)
+                at = np.argsort(s)
+                size_of = np.abs(kc[:p + 1, h // 2]) @ np.abs(q[starts[i] + j, h].astype(np.float64))
+                if len(at) > 1 and s[at[-1]] - s[at[-2]] < 2.0 ** -15 * size_of.max():
+                    continue
+                told += 1
+                # the lone weight is 2^(8 + the rounding of c s), itself rounded to f16 (half a step)
+                # while the f32 sum has it whole: attention_bound of a mass of |v|
+                lone = vc[at[-1], h // 2]
+                off = np.abs(got[starts[i] + j, h * 128:h * 128 + 128] - lone)
+                assert (off <= ck.attention_bound(lone, np.abs(lone))).all()
+    assert told > 100
+    tt.check()
+
+
+@pytest.mark.parametrize("q32", [False, True])
+@pytest.mark.parametrize("new,gqa", [(3, 1), (70, 4)])
+def test_scores_far_below_f32s_steps_then_ordinary_ones(tt, new, gqa, q32):
+    """Scores of -1e9 and less at a row's first positions, scores of a few units behind them, which
+    alone weigh."""
+    starts, spans, table, k, v = ck.batch(71, [new], [900 - new], 1, 32)
+    at = np.arange(900)
+    k[table[0, at // 32], 0, at % 32, 0] = 0
+    level = (starts, spans, table, k.copy(), v)
+    k[table[0, at[:700] // 32], 0, at[:700] % 32, 0] = -60000
+    q = np.random.default_rng(72).standard_normal((new, gqa, 128))
+    q[..., 0] = 60000
+    q = q.astype(np.float32 if q32 else np.float16)
+    b = (starts, spans, table, k, v)
+    got = attend(tt, q, b, 2.0)
+    want, mass = ck.attention(q, *b, 2.0, 0, np.zeros(got.shape))
+    assert (np.abs(got - want) <= ck.attention_bound(want, mass) + 2 * score_error(q, level, 2.0) * mass).all()
+    tt.check()
