@@ -388,11 +388,16 @@ TTS_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc
       "r"(a), "l"(b_desc), "r"(idesc), "r"(acc)
       : "memory");
 }
+// The first position that the row at `pos` sees (0 for rows before position 0). The comparison keeps
+// the difference in range: a window may be any size, a position as far below 0 as there are rows.
+TTS_DEV int ca_first(int pos, int window) {
+  return window > 0 && pos >= window ? pos + 1 - window : 0;
+}
 // First unit and number of units of a lane's work tile k (at least one: rows that see nothing are
 // written too).
 TTS_DEV void ca_units(int n, int pos0, CaDiv gqa, int window, int k, int* first, int* count) {
   const int t0 = k * kCaTile / gqa, t1 = min(n, (k * kCaTile + kCaTile - 1) / gqa + 1);
-  const int lo = window > 0 ? max(0, pos0 + t0 + 1 - window) : 0;
+  const int lo = ca_first(pos0 + t0, window);
   const int last = max(0, pos0 + t1 - 1) / kCaKeys;
   *first = lo / kCaKeys;
   *count = last - *first + 1;
@@ -441,7 +446,7 @@ __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, i
   const int tok = f / a.by_gqa, head = s.head * a.r.gqa + f - tok * a.r.gqa;
   const int pos = s.pos0 + tok;
   const int u0 = s.unit0 * kCaKeys, u1 = min(hi, (s.unit0 + s.units) * kCaKeys);
-  const int lo = a.r.window > 0 ? max(0, pos + 1 - a.r.window) : 0;
+  const int lo = ca_first(pos, a.r.window);
   const auto finite4 = [&](int p) {
     const long at = ca_pool_row(a, s.lane, s.head, p);
     if (at < 0) return true;
@@ -918,7 +923,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       w.work = __any_sync(0xffffffffu, w.live);
       const int tok = w.f / a.by_gqa;
       w.pos = w.live ? s.pos0 + tok : -1;
-      w.lo = r.window > 0 ? max(0, w.pos + 1 - r.window) : 0;
+      w.lo = ca_first(w.pos, r.window);
       w.rh = w.live ? ((s.row0 + tok) * r.n_kv + s.head - tok) * r.gqa + w.f : -1;
       return w;
     };

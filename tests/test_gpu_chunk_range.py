@@ -155,3 +155,20 @@ def test_scores_far_below_f32s_steps_then_ordinary_ones(tt, new, gqa, q32):
     want, mass = ck.attention(q, *b, 2.0, 0, np.zeros(got.shape))
     assert (np.abs(got - want) <= ck.attention_bound(want, mass) + 2 * score_error(q, level, 2.0) * mass).all()
     tt.check()
+
+
+@pytest.mark.parametrize("q32", [False, True])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 3, 2 ** 30, 5])
+def test_windows_of_any_size_over_rows_before_position_0(tt, window, q32):
+    """Lanes with (many) more new rows than positions beside ordinary ones."""
+    starts, spans, table, k, v = ck.batch(73, [3, 20, 300, 1], [0, 400, 10, 129], 2, 16)
+    spans[0], spans[2] = 0, 7
+    q = np.random.default_rng(74).standard_normal((324, 4, 128)).astype(np.float32 if q32 else np.float16)
+    b = (starts, spans, table, k, v)
+    got = attend(tt, q, b, window=window, out=torch.full((324, 512), 9.0, device="cuda", dtype=torch.float16))
+    wide = starts.astype(np.int64)  # numpy's int32 would wrap as well
+    want, mass = ck.attention(q, wide, spans, table, k, v, SCALE, window, np.zeros(got.shape))
+    slack = 2 * score_error(q, b, SCALE) * mass
+    assert (np.abs(got - want) <= ck.attention_bound(want, mass) + slack).all()
+    assert (got[:3] == 0).all() and (got[23:316] == 0).all()
+    tt.check()
