@@ -725,7 +725,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     CaSeg s;
     while (ok && (ok = next_seg(&s)) && s.units > 0) {
       const int last = min(s.n, (s.flat0 + kCaTile - 1) / a.by_gqa + 1);
-      const int hi = s.pos0 + last;  // positions from here on are seen by no row of the tile
+      // the tile's rows see positions lo .. hi - 1; boxes before or behind them are not loaded (their
+      // pages may be gone), and their values are zero
+      const int lo = ca_first(s.pos0 + s.flat0 / a.by_gqa, r.window), hi = s.pos0 + last;
       const int* table = r.block_table + (size_t)s.lane * r.max_blocks;
       const int end = min(hi, (s.unit0 + s.units) * kCaKeys);
       // this warp lane's box of the next unit: its position, block and (once read) page
@@ -734,11 +736,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       int blk = block(), page = wl < boxes && p < end ? table[blk] : -1;
       for (int j = 0; j < s.units; ++j) {
         const int p0 = (s.unit0 + j) * kCaKeys;
-        const bool seen = wl < boxes && p < hi, bad = seen && (page < 0 || page >= r.num_blocks);
+        const bool past = wl < boxes && p + a.box <= lo, seen = wl < boxes && p < hi && !past;
+        const bool bad = seen && (page < 0 || page >= r.num_blocks);
         const int row =
             seen && !bad ? (page * r.n_kv + s.head) * r.block_size + (p - blk * r.block_size) : -1;
         const unsigned load = __ballot_sync(0xffffffffu, row >= 0);
-        const unsigned zero = __ballot_sync(0xffffffffu, bad);
+        const unsigned flag = __ballot_sync(0xffffffffu, bad);
+        const unsigned zero = __ballot_sync(0xffffffffu, bad || (past && v));
         p += kCaKeys;
         blk = block();
         page = wl < boxes && p < end ? table[blk] : -1;  // on its way while this tile is loaded
@@ -753,8 +757,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             *reinterpret_cast<uint4*>(tile + ca_at(r0 + (e >> 4), e & 15)) =
                 make_uint4(0, 0, 0, 0);
         };
+        if (flag && wl == 0) atomicOr(r.err, kFlagPageRange);
         if (zero) {  // pages outside the pool read as zero
-          if (wl == 0) atomicOr(r.err, kFlagPageRange);
           for (unsigned m = zero; m; m &= m - 1) zero_rows((__ffs(m) - 1) * a.box, a.box);
           fence_proxy_async();
         }

@@ -172,3 +172,27 @@ def test_windows_of_any_size_over_rows_before_position_0(tt, window, q32):
     assert (np.abs(got - want) <= ck.attention_bound(want, mass) + slack).all()
     assert (got[:3] == 0).all() and (got[23:316] == 0).all()
     tt.check()
+
+
+@pytest.mark.parametrize("q32", [False, True])
+@pytest.mark.parametrize("page,window", [(8, 1), (8, 100), (16, 37), (24, 300), (64, 130), (128, 129), (32, 32)])
+def test_pages_before_the_window_may_be_gone(tt, page, window, q32):
+    """Block-table entries of pages that lie wholly before every row's window name no page of the
+    pool: nothing is reported and no row changes, with NaN among the values beside them too."""
+    new, held = [1, 1, 40, 1, 170, 3], [900, 333, 500, 129, 260, 700]
+    b = ck.batch(75, new, held, 2, page)
+    starts, spans, table, k, v = b
+    for i in range(6):
+        first = max(0, held[i] + 1 - window)  # the first position that a row of the lane sees
+        gone = np.arange(first // page)
+        table[i, gone] = np.where(gone % 3 == 0, -1, np.where(gone % 3 == 1, k.shape[0], 2 ** 30))
+        if first % page:
+            at = np.arange(first // page * page, first)
+            v[table[i, at // page], :, at % page] = np.nan
+    q = np.random.default_rng(76).standard_normal((int(starts[-1]), 4, 128)).astype(np.float32 if q32 else np.float16)
+    got = attend(tt, q, b, window=window)
+    tt.check()
+    want, mass = ck.attention(q, *b, SCALE, window, np.zeros(got.shape))
+    slack = 2 * score_error(q, (starts, spans, np.clip(table, 0, k.shape[0] - 1), k, v), SCALE) * mass
+    off = np.abs(got - want) - ck.attention_bound(want, mass) - slack
+    assert not np.isnan(got).any() and off.max() <= 0, (off.max(), np.argwhere(off > 0)[:4])
