@@ -181,6 +181,7 @@ struct CaSmem {
   // written again four runs later, when all warps have left it)
   uint8_t q_exp[kParts - 1 ? 2 : 1][128], few_exp[kCaSegs][32];
   uint32_t tmem;
+  uint32_t repaired;  // goes up with every row that was looked at again
 };
 
 template <int N>
@@ -240,14 +241,23 @@ TTS_DEV float ex2(float x) {
 
 // mbar_wait_warp with its bound (about 2 s) on the SM's own clock: the softmax and the MMAs hand
 // over to each other several times a unit, and reading the global timer on each hand-over cost more
-// than the hand-over.
-TTS_DEV bool ca_wait(uint64_t* bar, uint32_t parity, long long limit = 4000000000ll) {
+// than the hand-over. The bound starts anew while rows are being summed again (ca_repair, which ends
+// by itself), as that may take any time at long contexts.
+template <typename Smem>
+TTS_DEV bool ca_wait(Smem& S, uint64_t* bar, uint32_t parity, long long limit = 4000000000ll) {
   bool ok = mbar_try_wait(bar, parity);
   if (!ok) {
-    const long long t0 = clock64();
+    long long t0 = clock64();
+    uint32_t repaired = 0;  // (one bound more at first, where rows were before)
     do {
       ok = mbar_try_wait(bar, parity);
-    } while (!ok && clock64() - t0 < limit);
+      if (!ok && clock64() - t0 >= limit) {
+        const uint32_t now = *static_cast<volatile uint32_t*>(&S.repaired);
+        if (now == repaired) break;
+        repaired = now;
+        t0 = clock64();
+      }
+    } while (!ok);
   }
   return __all_sync(0xffffffffu, ok);
 }
@@ -421,66 +431,120 @@ TTS_DEV CaLane ca_lane(const ChunkAttnRequest& r, int i) {
   return ca_lane(r, r.row_start[i], r.row_start[i + 1], r.spans[i]);
 }
 
-template <typename TQ>
-TTS_DEV float ca_q(const CaArgs& a, int row, int head, int d) {
-  const float x =
-      float(static_cast<const TQ*>(a.r.q)[((size_t)row * a.r.n_kv * a.r.gqa + head) * 128 + d]);
-  return a.negate ? -x : x;
+// The pool row of a lane's position, -1 where the page is outside the pool.
+TTS_DEV int ca_pool_row(const CaArgs& a, int lane, int head, int pos) {
+  const int block = pos / a.by_page;
+  const int page = a.r.block_table[(size_t)lane * a.r.max_blocks + block];
+  if (page < 0 || page >= a.r.num_blocks) return -1;
+  return (page * a.r.n_kv + head) * a.r.block_size + (pos - block * a.r.block_size);
 }
 
-// The pool row of a lane's position, -1 where the page is outside the pool.
-TTS_DEV long ca_pool_row(const CaArgs& a, int lane, int head, int pos) {
-  const int page = a.r.block_table[(size_t)lane * a.r.max_blocks + pos / a.r.block_size];
-  if (page < 0 || page >= a.r.num_blocks) return -1;
-  return ((long)page * a.r.n_kv + head) * a.r.block_size + pos % a.r.block_size;
+// Eight elements of a query as f32.
+TTS_DEV void ca_load8(const float* p, float* x) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+TTS_DEV void ca_load8(const __half* p, float* x) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
 }
 
 // Positions a row does not see have weight 0, but an infinity or NaN among their values makes 0
 // times it NaN. Where a row's output is not finite, the warp looks at the values the row's units
 // held beyond what it sees and, if one is not finite, sums the row again over what it sees (dims
-// 4 lane .. + 3 of the result to each warp lane). Never reached by finite caches.
+// 4 lane .. + 3 of the result to each warp lane). Never reached by finite caches. Half a warp takes
+// a position, 16 positions' rows are on their way at once: a tile of such rows over a long cache
+// should not keep the CTA for long (37 lanes of 128 rows of 8 heads over 8192 positions, the last of
+// them NaN: 34 ms, one position at a time 185).
 template <typename TQ>
 __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, int hi, CaAim aim,
                                        float4* o) {
-  const int wl = threadIdx.x & 31;
+  const int wl = threadIdx.x & 31, half = wl >> 4, d0 = (wl & 15) * 8;
   const int tok = f / a.by_gqa, head = s.head * a.r.gqa + f - tok * a.r.gqa;
   const int pos = s.pos0 + tok;
   const int u0 = s.unit0 * kCaKeys, u1 = min(hi, (s.unit0 + s.units) * kCaKeys);
   const int lo = ca_first(pos, a.r.window);
-  const auto finite4 = [&](int p) {
-    const long at = ca_pool_row(a, s.lane, s.head, p);
-    if (at < 0) return true;
-    const uint2 u = *reinterpret_cast<const uint2*>(a.r.v_pool + at * 128 + wl * 4);
-    const uint32_t e = 0x7c007c00u;  // an all-ones exponent in either half
-    return (u.x & e & 0xffffu) != 0x7c00u && (u.x & e) >> 16 != 0x7c00u &&
-           (u.y & e & 0xffffu) != 0x7c00u && (u.y & e) >> 16 != 0x7c00u;
+  // the pool rows of 32 positions from p on, one a warp lane, -1 from `end` on
+  const auto rows_at = [&](int p, int end) {
+    return p + wl < end ? ca_pool_row(a, s.lane, s.head, p + wl) : -1;
+  };
+  const auto piece = [&](const __half* pool, int row) {
+    return row < 0 ? make_uint4(0, 0, 0, 0)
+                   : *reinterpret_cast<const uint4*>(pool + (size_t)row * 128 + d0);
   };
   bool clean = true;
-  for (int p = u0; p < min(lo, u1); ++p) clean = clean && finite4(p);
-  for (int p = max(u0, pos + 1); p < u1; ++p) clean = clean && finite4(p);
+  const auto look = [&](int from, int end) {
+    for (int p = from; p < end; p += 32) {
+      const int at = rows_at(p, end);
+#pragma unroll 4
+      for (int i = 0; i < 32; i += 2) {
+        const uint4 v = piece(a.r.v_pool, __shfl_sync(0xffffffffu, at, i + half));
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)  // an all-ones exponent in either half
+          clean = clean && (u[e] & 0x7c00u) != 0x7c00u && (u[e] >> 16 & 0x7c00u) != 0x7c00u;
+      }
+    }
+  };
+  look(u0, min(lo, u1));
+  look(max(u0, pos + 1), u1);
   if (__all_sync(0xffffffffu, clean)) return false;
-  float q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = ca_q<TQ>(a, s.row0 + tok, head, wl * 4 + i);
+  float q[8];
+  ca_load8(static_cast<const TQ*>(a.r.q) +
+               ((size_t)(s.row0 + tok) * a.r.n_kv * a.r.gqa + head) * 128 + d0, q);
+  float up = a.negate ? -1.f : 1.f;
   if (sizeof(TQ) == 4) {  // as the scores' queries were
-    const float most = fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3])));
-    const float up =
-        ca_scale_up(ca_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(most))));
+    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] *= up;
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(q[e]));
+    up *= ca_scale_up(ca_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(most))));
   }
-  *o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = max(u0, lo); p < min(u1, pos + 1); ++p) {
-    const long at = ca_pool_row(a, s.lane, s.head, p);
-    if (at < 0) continue;
-    const __half2* k = reinterpret_cast<const __half2*>(a.r.k_pool + at * 128 + wl * 4);
-    const __half2* v = reinterpret_cast<const __half2*>(a.r.v_pool + at * 128 + wl * 4);
-    const float2 k0 = __half22float2(k[0]), k1 = __half22float2(k[1]);
-    const float x = warp_sum(q[0] * k0.x + q[1] * k0.y + q[2] * k1.x + q[3] * k1.y);
-    const float w = ex2(fmaf(x, aim.c, aim.bias));
-    const float2 v0 = __half22float2(v[0]), v1 = __half22float2(v[1]);
-    o->x += w * v0.x, o->y += w * v0.y, o->z += w * v1.x, o->w += w * v1.y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] *= up;
+  float sum[8] = {};
+  const int end = min(u1, pos + 1);
+  for (int p = max(u0, lo); p < end; p += 32) {
+    const int at = rows_at(p, end);
+#pragma unroll 1
+    for (int i0 = 0; i0 < 32; i0 += 16) {
+      uint4 k[8], v[8];
+      int row[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        row[i] = __shfl_sync(0xffffffffu, at, i0 + 2 * i + half);
+        k[i] = piece(a.r.k_pool, row[i]);
+        v[i] = piece(a.r.v_pool, row[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float x[8], y = 0.f;
+        ca_load8(reinterpret_cast<const __half*>(&k[i]), x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y = fmaf(q[e], x[e], y);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) y += __shfl_xor_sync(0xffffffffu, y, d);
+        const float w = row[i] < 0 ? 0.f : ex2(fmaf(y, aim.c, aim.bias));
+        ca_load8(reinterpret_cast<const __half*>(&v[i]), x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = fmaf(w, x[e], sum[e]);
+      }
+    }
   }
+  float out[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float lower = sum[e] + __shfl_xor_sync(0xffffffffu, sum[e], 16);
+    const float upper = sum[e + 4] + __shfl_xor_sync(0xffffffffu, sum[e + 4], 16);
+    const float even = __shfl_sync(0xffffffffu, lower, wl >> 1);
+    const float odd = __shfl_sync(0xffffffffu, upper, wl >> 1);
+    out[e] = wl & 1 ? odd : even;
+  }
+  *o = make_float4(out[0], out[1], out[2], out[3]);
   return true;
 }
 
@@ -611,6 +675,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     }
     fence_barrier_init();
     if (wl == 0) {
+      S.repaired = 0;
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
     }
@@ -631,7 +696,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
   uint32_t seg_phase = 0;
   // every role reads the work in order and frees its slot at once
   const auto next_seg = [&](CaSeg* s) {
-    if (!ca_wait(&S.seg_full[seg_slot], seg_phase)) return false;
+    if (!ca_wait(S, &S.seg_full[seg_slot], seg_phase)) return false;
     *s = S.seg[seg_slot];
     __syncwarp();
     if (wl == 0) mbar_arrive(&S.seg_empty[seg_slot]);
@@ -657,7 +722,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       buf = ca_q_buffer(few, was_few, buf);
       was_few = few;
       if (!few || i == 0) return;
-      if (free >= 0) ok = ca_wait(&S.seg_done[free % kCaSegs], (free / kCaSegs) & 1);
+      if (free >= 0) ok = ca_wait(S, &S.seg_done[free % kCaSegs], (free / kCaSegs) & 1);
       if (!ok) return;
       const int f = s.flat0 + wl, tok = f / a.by_gqa;
       ca_copy_q(S.q[buf], static_cast<const TQ*>(r.q),
@@ -694,7 +759,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           p.valid = 1;
         }
       }
-      ok = ca_wait(&S.seg_empty[seg_slot], seg_phase ^ 1);
+      ok = ca_wait(S, &S.seg_empty[seg_slot], seg_phase ^ 1);
       if (!ok) break;
       if (wl == 0) {
         S.seg[seg_slot] = s;
@@ -748,7 +813,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         page = wl < boxes && p < end ? table[blk] : -1;  // on its way while this tile is loaded
         const bool tail = v && p0 + kCaKeys > hi;
         uint64_t* full = &S.full[base + slot];
-        ok = ca_wait(&S.empty[base + slot], phase ^ 1);
+        ok = ca_wait(S, &S.empty[base + slot], phase ^ 1);
         if (!ok) break;
         uint8_t* tile = S.ring[base + slot];
         if (wl < kCaKeys / 8) reinterpret_cast<int*>(S.box_row[v])[wl] = row;
@@ -785,7 +850,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         __syncwarp();
         if (tail) {
           // rows that nothing sees: their stale bits times a weight of 0 could be NaN
-          ok = ca_wait(&S.tail, tail_phase);
+          ok = ca_wait(S, &S.tail, tail_phase);
           tail_phase ^= 1;
           if (!ok) break;
           const int keep = max(hi - p0, 0);
@@ -798,7 +863,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       }
     }
     if (!ok)  // bounded: copies still on their way
-      for (int i = 0; i < ring; ++i) ca_wait(&S.full[base + i], phase, 200000000ll);
+      for (int i = 0; i < ring; ++i) ca_wait(S, &S.full[base + i], phase, 200000000ll);
   } else if (warp == 9) {
     // ---- the MMAs. Tile by tile and unit by unit: O_t += P_t.V(j), then S_t = Q_t.K(j + 1) over
     // the P just read (MMAs of one thread run in the order of their issue).
@@ -842,10 +907,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       uint64_t* const done = &S.seg_done[run++ % kCaSegs];  // after the run's last scores
       for (int b = 0; b < 2 && ok; ++b) {
         if (one && b >= s.units) break;
-        if (b == 0 || one) ok = ca_wait(&S.full[k_slot], k_phase);
+        if (b == 0 || one) ok = ca_wait(S, &S.full[k_slot], k_phase);
         if (ok && (b == 0 || !one)) {
           const int from = one ? buf : b;
-          ok = ca_wait(&S.q_full[from], q_phase[from]);
+          ok = ca_wait(S, &S.q_full[from], q_phase[from]);
           q_phase[from] ^= 1;
         }
         if (!ok) break;
@@ -860,14 +925,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       }
       for (int j = 0; j < s.units && ok; ++j) {
         const bool more = j + ahead < s.units;
-        ok = ca_wait(&S.full[kK + v_slot], v_phase);
+        ok = ca_wait(S, &S.full[kK + v_slot], v_phase);
         const uint64_t vd = ca_desc(v_desc, v_slot * kTile16);
         for (int b = one ? j & 1 : 0; b < (one ? (j & 1) + 1 : 2) && ok; ++b) {
           const auto values = [&](int kk) {
             umma_f16_ts(tmem + 256 + b * 128, tmem + b * 128 + kk * 8,
                         ca_desc(vd, kk * (4096 / 16)), idesc_o, j >= ahead || kk > 0);
           };
-          ok = ca_wait(&S.h_full[b], p_phase[b]);
+          ok = ca_wait(S, &S.h_full[b], p_phase[b]);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -876,9 +941,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             umma_commit(&S.h_done[b]);
           }
           __syncwarp();
-          ok = ca_wait(&S.p_full[b], p_phase[b]);
+          ok = ca_wait(S, &S.p_full[b], p_phase[b]);
           p_phase[b] ^= 1;
-          if (ok && more && (b == 0 || one)) ok = ca_wait(&S.full[k_slot], k_phase);
+          if (ok && more && (b == 0 || one)) ok = ca_wait(S, &S.full[k_slot], k_phase);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -905,7 +970,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     if (!ok) {  // bounded: MMAs still running
       if (elect_one()) umma_commit(&S.drain);
       __syncwarp();
-      ca_wait(&S.drain, 0, 200000000ll);
+      ca_wait(S, &S.drain, 0, 200000000ll);
     }
     }
   } else {
@@ -943,7 +1008,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       float c = a.c;      // of scores as they come from the MMAs
       const int step0 = w.one ? tl : 0, steps = w.one ? 2 : 1;
       for (int j = step0; j < s.units; j += steps) {
-        ok = ca_wait(&S.s_full[tl], s_phase);
+        ok = ca_wait(S, &S.s_full[tl], s_phase);
         s_phase ^= 1;
         if (!ok) break;
         tc_fence_after();
@@ -991,7 +1056,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 sum *= keep;
                 fresh = __any_sync(0xffffffffu, ref == -INFINITY);
                 if (h > 0) {  // the first half's MMAs; before that, S(j) came after all others
-                  ok = ca_wait(&S.h_done[tl], s_phase ^ 1);
+                  ok = ca_wait(S, &S.h_done[tl], s_phase ^ 1);
                   if (!ok) break;
                   tc_fence_after();
                 }
@@ -1043,7 +1108,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       if (load && !w.one)
         ca_copy_q(S.q[tl], static_cast<const TQ*>(r.q), wn.rh, (warp & 3) * 32);
       if (step0 < s.units) {
-        ok = ca_wait(&S.o_full[tl], o_phase);
+        ok = ca_wait(S, &S.o_full[tl], o_phase);
         o_phase ^= 1;
         if (!ok) break;
         tc_fence_after();
@@ -1058,9 +1123,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (wl == 0) mbar_arrive(&S.x_full);
-          ok = ca_wait(&S.x_empty, x_phase);
+          ok = ca_wait(S, &S.x_empty, x_phase);
         } else {
-          ok = ca_wait(&S.x_full, x_phase);
+          ok = ca_wait(S, &S.x_full, x_phase);
           tc_fence_after();
           if (s.units > 1) {
             const float ref1 = S.x_ref[lane_row], top = max3(ref, ref1, ref1);
@@ -1156,7 +1221,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           const int sf = __shfl_sync(0xffffffffu, w.f, src);
           const int spr = __shfl_sync(0xffffffffu, w.pr, src);
           const int at = __shfl_sync(0xffffffffu, w.rh, src);
-          if (!ca_repair<TQ>(a, s, sf, hi, saim, &y)) continue;
+          const bool summed = ca_repair<TQ>(a, s, sf, hi, saim, &y);
+          if (wl == 0) atomicAdd(&S.repaired, 1u);
+          if (!summed) continue;
           __syncwarp();  // after the row's own stores
           if (whole) {
             __half2* h = reinterpret_cast<__half2*>(r.out + (size_t)at * 128 + wl * 4);

@@ -196,3 +196,37 @@ def test_pages_before_the_window_may_be_gone(tt, page, window, q32):
     slack = 2 * score_error(q, (starts, spans, np.clip(table, 0, k.shape[0] - 1), k, v), SCALE) * mass
     off = np.abs(got - want) - ck.attention_bound(want, mass) - slack
     assert not np.isnan(got).any() and off.max() <= 0, (off.max(), np.argwhere(off > 0)[:4])
+
+
+@pytest.mark.parametrize("q32", [False, True])
+@pytest.mark.parametrize("window", [0, 130000])
+def test_values_not_finite_beside_long_spans(tt, window, q32):
+    """A NaN that one row of a tile sees, over 131072 positions: the tile's other rows are summed
+    again, in every lane, without a wait of the CTA's other warps running out."""
+    lanes, new, span, page = 74, 128, 131072, 64
+    g = torch.Generator(device="cuda").manual_seed(77)
+    k, v = (torch.randn(span // page, 2, page, 128, device="cuda", generator=g).half() for _ in range(2))
+    v += 2  # so that a sum of them is not near 0
+    table = torch.arange(span // page, dtype=torch.int32, device="cuda").repeat(lanes, 1)
+    bad = max(0, span - new + 1 - window) if window else span - 1  # of the first row, or the last
+    v[bad // page, :, bad % page] = float("nan")
+    one = torch.randn(new, 4, 128, device="cuda", generator=g)
+    one = one if q32 else one.half()
+    starts = torch.arange(lanes + 1, dtype=torch.int32, device="cuda") * new
+    spans = torch.full((lanes,), span, dtype=torch.int32, device="cuda")
+    got = tt.attn.chunk_attention(one.repeat(lanes, 1, 1), starts, spans, tt.attn.paged_cache(k, v, table), SCALE,
+                                  window).reshape(lanes, new, 4, 128)
+    tt.check()
+    at, p = torch.arange(span, device="cuda"), torch.arange(span - new, span, device="cuda")[:, None]
+    seen = (at <= p) & (at > p - window if window else at >= 0)
+    alone = 0 if window else new - 1
+    keep = [r for r in range(new) if r != alone]
+    for h in range(4):
+        kc, vc = (t[:, h // 2].reshape(span, 128).double() for t in (k, v))
+        vc[bad] = 0
+        w = torch.softmax((one[:, h].double() @ kc.T * SCALE).masked_fill(~seen, -torch.inf), 1)
+        want, mass = w @ vc, w @ vc.abs()
+        # attention_bound, and f32 sums of 65536 products (half a warp's) and 2048 weights in a row
+        bound = (ck.F16 + 2.0 ** -13 + 67584 * ck.F32) * mass + ck.F16 * want.abs() + 2.0 ** -25
+        assert (got[:, :, h].double() - want).abs().sub(bound)[:, keep].max() <= 0
+        assert torch.isnan(got[:, alone, h]).all()
