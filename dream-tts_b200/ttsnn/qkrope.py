@@ -109,7 +109,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
 
     def whole(t):
         row, head, one = t.stride()
-        return (one == 1 and head == hd and row % 8 == 0 and row >= heads * hd
+        return (one == 1 and head == hd and row % 8 == 0 and heads * hd <= row < 2 ** 31
                 and t.data_ptr() % 16 == 0)
 
     if out is None:

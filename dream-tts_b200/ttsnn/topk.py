@@ -76,8 +76,9 @@ def sample_filtered(logits: torch.Tensor, draws: torch.Tensor, temperature=None,
     of one per row. int32 [rows], -1 where no id can be picked (tts_filter_sample)."""
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.float16):
         raise ValueError("sample_filtered: logits must be [rows, n], f32 or f16")
-    x = logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
-    rows, n = x.shape
+    rows, n = logits.shape
+    # (the library's row stride is an int)
+    x = logits if logits.stride(1) == 1 and n <= logits.stride(0) < 2 ** 31 else logits.contiguous()
     d = _per_row(draws, rows, torch.float32, x.device, "draws")
     if d is None:
         raise ValueError("sample_filtered: draws are needed")
