@@ -60,10 +60,14 @@ def _per_row(v, rows: int, dtype: torch.dtype, device: torch.device, name: str):
     """A setting for every row: None, one value for all, or a tensor of one per row."""
     if v is None:
         return None
+    whole = dtype == torch.int32  # any number keeps its meaning: -1 is off, so is 2^30 for any row
     if not isinstance(v, torch.Tensor):
+        v = min(max(v, -1), 2 ** 30) if whole else v
         return torch.full((rows,), v, dtype=dtype, device=device)
     if v.numel() != rows or v.device != device:
         raise ValueError(f"sample_filtered: {name} must hold one value per row, on {device}")
+    if whole and v.dtype != dtype:
+        v = v.to(torch.int64).clamp(-1, 2 ** 30)
     return as_type(v, dtype)
 
 
