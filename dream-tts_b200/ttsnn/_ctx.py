@@ -44,6 +44,13 @@ def as_type(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+def packed(t: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """t as contiguous `dtype` (None: its own) from a 16-byte boundary on."""
+    t = t.contiguous() if dtype is None else as_type(t, dtype)
+    # (torch calls a view that starts anywhere contiguous, and then hands out itself)
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 def ptr(t: torch.Tensor | None) -> C.c_void_p:
     return C.c_void_p(0 if t is None else t.data_ptr())
 

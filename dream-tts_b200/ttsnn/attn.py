@@ -6,7 +6,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from ._ctx import ctx_of, ptr, stream, stream_of
+from ._ctx import ctx_of, packed, ptr, stream, stream_of
 from .qkrope import chunk_batch, contiguous_cache, same_device
 
 
@@ -84,7 +84,7 @@ def chunk_attention(q: torch.Tensor, row_start: torch.Tensor, spans: torch.Tenso
         raise ValueError("chunk_attention: out must be contiguous f16 [rows, heads * 128]")
     if rows == 0:
         return out
-    qc = q.contiguous()
+    qc = packed(q)
     c = ctx_of(q)
     # from torch's allocator, so that calls on several streams or in several graphs have their own
     size = _workspace.get(q.device.index)

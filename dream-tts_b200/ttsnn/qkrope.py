@@ -6,7 +6,7 @@ import ctypes as C
 import torch
 
 from . import _lib as L
-from ._ctx import as_type, ctx_of, ptr, stream, stream_of
+from ._ctx import ctx_of, packed, ptr, stream, stream_of
 
 
 def eligible(qkv: torch.Tensor, k_cache: torch.Tensor, head_dim: int) -> bool:
@@ -90,7 +90,7 @@ def same_device(op: str, x: torch.Tensor, *others: torch.Tensor | None) -> None:
 def _tables(op: str, cos: torch.Tensor, sin: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if cos.shape != sin.shape or cos.dim() != 2:
         raise ValueError(f"{op}: cos and sin must be [positions, rotary_dim / 2] both")
-    return as_type(cos, torch.float32), as_type(sin, torch.float32)
+    return packed(cos, torch.float32), packed(sin, torch.float32)
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -108,9 +108,12 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
     c, s = _tables("rotary", cos, sin)
 
     def whole(t):
-        row, head, one = t.stride()
-        return (one == 1 and head == hd and row % 8 == 0 and heads * hd <= row < 2 ** 31
-                and t.data_ptr() % 16 == 0)
+        row, head, one = t.stride()  # of a dimension of one entry it says nothing
+        return (one == 1 and (head == hd or heads == 1) and t.data_ptr() % 16 == 0
+                and (rows == 1 or row % 8 == 0 and heads * hd <= row < 2 ** 31))
+
+    def pitch(t):
+        return t.stride(0) if rows > 1 else heads * hd
 
     if out is None:
         y = x.new_empty((rows, heads, hd))
@@ -121,11 +124,11 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: tor
         y = out
     if rows == 0:
         return y
-    xc = x if whole(x) else x.contiguous()
+    xc = x if whole(x) else packed(x)
     length, pairs = c.shape
     L.call("tts_rotary", ctx_of(x), xc.data_ptr(), x.dtype == torch.float16, rows, heads, hd,
-           xc.stride(0), positions.data_ptr(), c.data_ptr(), s.data_ptr(), length, 2 * pairs,
-           bool(interleaved), y.data_ptr(), y.stride(0), stream_of(x))
+           pitch(xc), positions.data_ptr(), c.data_ptr(), s.data_ptr(), length, 2 * pairs,
+           bool(interleaved), y.data_ptr(), pitch(y), stream_of(x))
     return y
 
 
@@ -157,8 +160,8 @@ def rotary_append(qkv: torch.Tensor, heads: int, row_start: torch.Tensor, spans:
         q = out
     if rows == 0:
         return q
-    x = qkv.contiguous()
-    nm = None if norms is None else as_type(norms, torch.float32)
+    x = packed(qkv)
+    nm = None if norms is None else packed(norms, torch.float32)
     L.call("tts_rotary_append", ctx_of(x), x.data_ptr(), int(x.dtype == torch.float16), int(heads),
            C.byref(b), None if nm is None else nm.data_ptr(), float(eps), c.data_ptr(),
            s.data_ptr(), c.shape[0], 2 * c.shape[1], int(interleaved), C.byref(kv), q.data_ptr(),

@@ -95,5 +95,5 @@ def sample_filtered(logits: torch.Tensor, draws: torch.Tensor, temperature=None,
     if rows == 0:
         return out
     L.call("tts_filter_sample", ctx_of(x), x.data_ptr(), int(x.dtype == torch.float16), rows, n,
-           x.stride(0), d.data_ptr(), C.byref(how), out.data_ptr(), stream_of(x))
+           x.stride(0) if rows > 1 else 0, d.data_ptr(), C.byref(how), out.data_ptr(), stream_of(x))
     return out

@@ -72,3 +72,78 @@ def test_top_k_of_any_size(monkeypatch, calls, top_k, want):
     topk.sample_filtered(torch.zeros(4, 9), torch.zeros(4), top_k=top_k)
     for g, w in zip(got, want, strict=True):
         assert g <= 0 if w == -1 else g >= w if w == 2 ** 18 else w is None and (g <= 0 or g >= 2 ** 18) or g == w
+
+
+def off_by(n, *shape, dtype=torch.float32):
+    """A contiguous tensor `n` elements behind a 16-byte boundary."""
+    t = torch.randn(n + 64 + int(np.prod(shape)), generator=torch.Generator().manual_seed(len(shape)))
+    t = t.to(dtype)
+    skip = (-t.data_ptr() % 16) // t.element_size() + n
+    return t[skip:skip + int(np.prod(shape))].view(*shape)
+
+
+def held(monkeypatch, name, take):
+    """take(args) of the next call of `name`, read while its tensors live."""
+    got = []
+
+    def call(called, *args):
+        assert called == name
+        got.append(take(args))
+
+    monkeypatch.setattr(L, "call", call)
+    return got
+
+
+def f32(pointer, n):
+    assert pointer % 16 == 0
+    return values(pointer, C.c_float, n)
+
+
+def lane(n):
+    kv = attn.paged_cache(torch.zeros(2, 1, 16, 128).half(), torch.zeros(2, 1, 16, 128).half(),
+                          torch.zeros(1, 2, dtype=torch.int32))
+    return torch.tensor([0, n], dtype=torch.int32), torch.tensor([n], dtype=torch.int32), kv
+
+
+@pytest.mark.parametrize("off", [0, 1, 3])
+def test_inputs_that_start_between_16_byte_boundaries(monkeypatch, calls, off):
+    """Contiguous views at an odd offset are brought to a boundary, not refused."""
+    x, cos, sin = off_by(off, 3, 2, 16), off_by(off, 9, 8), off_by(off, 9, 8)
+    got = held(monkeypatch, "tts_rotary", lambda a: [f32(a[1], 96), f32(a[8], 72), f32(a[9], 72)])
+    qkrope.rotary(x, torch.zeros(3, dtype=torch.int32), cos, sin)
+    for g, t in zip(got[0], (x, cos, sin), strict=True):
+        assert np.array_equal(g, t.numpy().ravel())
+    starts, spans, kv = lane(3)
+    qkv, norms = off_by(off, 3, 3 * 128), off_by(off, 2, 128)
+    got = held(monkeypatch, "tts_rotary_append", lambda a: [f32(a[1], 3 * 384), f32(a[5], 256), f32(a[7], 72),
+                                                           f32(a[8], 72)])
+    qkrope.rotary_append(qkv, 1, starts, spans, cos, sin, kv, norms=norms)
+    for g, t in zip(got[0], (qkv, norms, cos, sin), strict=True):
+        assert np.array_equal(g, t.numpy().ravel())
+    q = off_by(off, 3, 2, 128)
+    monkeypatch.setitem(attn._workspace, q.device.index, 64)
+    got = held(monkeypatch, "tts_chunk_attention", lambda a: f32(a[1], 768))
+    attn.chunk_attention(q, starts, spans, kv, 1.0)
+    assert np.array_equal(got[0], q.numpy().ravel())
+
+
+def test_strides_of_one_row_or_head_say_nothing(monkeypatch, calls):
+    """A dimension of one entry may have any stride, torch calls such a tensor contiguous."""
+    column = torch.randn(100, 1).t()
+    assert column.stride() == (1, 1) and column.is_contiguous()
+    got = held(monkeypatch, "tts_filter_sample", lambda a: (a[5], values(a[1], C.c_float, 100)))
+    topk.sample_filtered(column, torch.zeros(1))
+    assert got[0][0] in (0, 100) and np.array_equal(got[0][1], column[0].numpy())
+    cos, sin, pos = torch.zeros(9, 8), torch.zeros(9, 8), torch.zeros(1, dtype=torch.int32)
+    for x in (torch.randn(40)[:32].as_strided((1, 2, 16), (3, 16, 1)),  # one row
+              torch.randn(9, 5, 16)[:1, :1], torch.randn(40).as_strided((1, 1, 16), (7, 5, 1))):
+        n = x.numel()
+        got = held(monkeypatch, "tts_rotary", lambda a: (a[6], a[14], f32(a[1], n)))
+        out = torch.empty(48).as_strided(x.shape, (5, 16 if x.shape[1] > 1 else 3, 1))
+        for y in (None, x, out):
+            qkrope.rotary(x, pos, cos, sin, out=y)
+        assert all(g[0] == g[1] == n and np.array_equal(g[2], x.numpy().ravel()) for g in got) and len(got) == 3
+    x = torch.randn(5, 9, 16)[:, :1]  # several rows of one head: still strided
+    got = held(monkeypatch, "tts_rotary", lambda a: (a[6], a[14]))
+    qkrope.rotary(x, torch.zeros(5, dtype=torch.int32), cos, sin)
+    assert got == [(144, 16)]

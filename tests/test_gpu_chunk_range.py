@@ -230,3 +230,43 @@ def test_values_not_finite_beside_long_spans(tt, window, q32):
         bound = (ck.F16 + 2.0 ** -13 + 67584 * ck.F32) * mass + ck.F16 * want.abs() + 2.0 ** -25
         assert (got[:, :, h].double() - want).abs().sub(bound)[:, keep].max() <= 0
         assert torch.isnan(got[:, alone, h]).all()
+
+
+def test_unaligned_and_one_row_views(tt):
+    """Views that start between 16-byte boundaries, and single rows and heads of any stride, give
+    what their copies give."""
+    off = lambda t, n=1: torch.cat([t.new_zeros(n), t.flatten()])[n:].view(t.shape)
+    g = torch.Generator(device="cuda").manual_seed(79)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    cos, sin = (dev(t) for t in ck.tables(90, 64))
+    pos = torch.arange(5, dtype=torch.int32, device="cuda") * 7
+    for x in (rand(5, 3, 64), rand(5, 3, 64).half()):
+        want = tt.qkrope.rotary(x, pos, cos, sin)
+        assert torch.equal(tt.qkrope.rotary(off(x), pos, off(cos), off(sin, 3)), want)
+        assert torch.equal(tt.qkrope.rotary(x.flatten()[64:256].as_strided((1, 3, 64), (5, 64, 1)), pos[:1], cos, sin),
+                           tt.qkrope.rotary(x.flatten()[64:256].clone().view(1, 3, 64), pos[:1], cos, sin))
+        assert torch.equal(tt.qkrope.rotary(x[:, 1:2], pos, cos, sin), want[:, 1:2])
+    starts, spans, table, k, v = ck.batch(80, [5], [20], 1, 8)
+    sd, pd, norms = dev(starts), dev(spans), rand(2, 128)
+    for x in (rand(5, 4 * 128), rand(5, 4 * 128).half()):
+        out = []
+        for qkv, c, s, w in ((x, cos, sin, norms), (off(x), off(cos), off(sin), off(norms, 2))):
+            kv = tt.attn.paged_cache(dev(k), dev(v), dev(table))
+            q = tt.qkrope.rotary_append(qkv, 2, sd, pd, c, s, kv, norms=w)
+            out += [q, kv.keep[0], kv.keep[1], tt.attn.chunk_attention(off(q) if qkv is not x else q, sd, pd, kv, SCALE)]
+        assert all(torch.equal(a, b) for a, b in zip(out[:4], out[4:], strict=True))
+    logits = rand(300, 1).t()
+    u = torch.full((1,), 0.6, device="cuda")
+    assert torch.equal(tt.topk.sample_filtered(logits, u), tt.topk.sample_filtered(logits.clone().reshape(1, 300), u))
+    tt.check()
+
+
+def test_filtered_draw_over_rows_far_apart(tt):
+    """A row stride past 31 bits."""
+    flat = torch.zeros(2 ** 31 + 4096, dtype=torch.float16, device="cuda")
+    x = flat.as_strided((2, 1000), (2 ** 31 + 8, 1))
+    x.copy_(torch.randn(2, 1000, device="cuda", generator=torch.Generator(device="cuda").manual_seed(81)))
+    u = torch.tensor([0.3, 0.8], device="cuda")
+    want = ck.sample(x.cpu().numpy(), u.cpu().numpy(), top_k=np.array([40, 0]))
+    got = tt.topk.sample_filtered(x, u, top_k=torch.tensor([40, 2 ** 40], device="cuda"))
+    assert np.array_equal(got.cpu().numpy(), want)
