@@ -218,8 +218,9 @@ __global__ void __launch_bounds__(kRotThreads, 3) rotary_append_kernel(const Rot
     const int lane = chunk_lane_of(starts, a.lanes, row);
     const int span = a.spans[lane];
     const int pos = span - (starts[lane + 1] - row);
-    if (span > cap || pos < 0 || pos >= a.rope_len) {
-      if (wl == 0) atomicOr(a.err, kFlagRopeRange);
+    const bool outside = span < 0 || span > cap || pos >= a.rope_len;
+    if (outside || pos < 0) {  // (a row before position 0 has no place: nothing is wrong with it)
+      if (outside && wl == 0) atomicOr(a.err, kFlagRopeRange);
       continue;
     }
     float c[4], sn[4];

@@ -139,7 +139,8 @@ def rotary_append(qkv: torch.Tensor, heads: int, row_start: torch.Tensor, spans:
     """A ragged chunk's rows `qkv [rows, (heads + 2 n_kv) * 128]` (f32 or f16): the QK-norm if
     `norms [2, 128]` is given, the rotation at each row's position, K and V into the pages; the
     rotated q `[rows, heads, 128]` is returned, f16 or f32 (or written to `out`). Lane i's rows
-    are row_start[i] .. row_start[i + 1] and spans[i] the positions it holds once they are in."""
+    are row_start[i] .. row_start[i + 1] and spans[i] the positions it holds once they are in; rows
+    before position 0 (more of them than spans[i]) are left out, of q too."""
     if qkv.dim() != 2 or qkv.dtype not in (torch.float32, torch.float16):
         raise ValueError("rotary_append: qkv must be [rows, width], f32 or f16")
     rows = qkv.shape[0]

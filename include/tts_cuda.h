@@ -254,10 +254,11 @@ TTS_API tts_status tts_filter_sample(tts_ctx* ctx, const void* logits, int logit
  * New rows of several lanes at once over a paged cache: chunks of long prompts, lanes of one
  * token each, or both together. Lane i's rows are row_start[i] .. row_start[i + 1] - 1 of the
  * call's row buffers (none is fine) and spans[i] the positions it holds once they are in, so row
- * j of its n sits at position spans[i] - n + j. Rows outside [row_start[0], row_start[lanes])
- * are left as they are. row_start int32 [lanes + 1] and spans int32 [lanes] are device memory:
+ * j of its n sits at position spans[i] - n + j. Rows before position 0 (more new rows than spans
+ * says) have no place in the cache: the append leaves them out, their attention is 0. Rows outside
+ * [row_start[0], row_start[lanes]) are left as they are. row_start int32 [lanes + 1] and spans int32 [lanes] are device memory:
  * row starts that descend or leave [0, rows] void the whole call (nothing is written), both that
- * and a span beyond the block table (its lane's rows are skipped) are reported by
+ * and a span below 0 or beyond the block table (its lane's rows are skipped) are reported by
  * tts_ctx_check. lanes <= 1024. No counterpart in the reference, whose Stack::forward takes one
  * length for the whole batch (crates/qwen3tts/src/qwen3.rs:294-467). */
 typedef struct tts_chunk_batch {
@@ -283,8 +284,9 @@ TTS_API tts_status tts_rotary(tts_ctx* ctx, const void* x, int x_f16, int rows, 
 /* tts_qk_rope_append for a ragged chunk: qkv f32 or f16 [rows][(heads + 2 n_kv) * 128]; the
  * QK-norm when `norms` is given (f32 [2][128], q's then k's weight, over the whole head), then
  * the rotation of tts_rotary at each row's position; q f32 or f16 [rows][heads][128] out (apart
- * from qkv), K and V (f16) into the pages (any page size). A position outside the tables or a
- * page outside the pool skips its row and is reported by tts_ctx_check. */
+ * from qkv), K and V (f16) into the pages (any page size). A position behind the tables or a
+ * page outside the pool skips its row and is reported by tts_ctx_check; rows that are skipped, those
+ * before position 0 too, leave q as it is. */
 TTS_API tts_status tts_rotary_append(tts_ctx* ctx, const void* qkv, int qkv_f16, int heads,
                                      const tts_chunk_batch* batch, const float* norms, float eps,
                                      const float* cos_t, const float* sin_t, int rope_len,

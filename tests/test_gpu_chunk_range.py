@@ -270,3 +270,34 @@ def test_filtered_draw_over_rows_far_apart(tt):
     want = ck.sample(x.cpu().numpy(), u.cpu().numpy(), top_k=np.array([40, 0]))
     got = tt.topk.sample_filtered(x, u, top_k=torch.tensor([40, 2 ** 40], device="cuda"))
     assert np.array_equal(got.cpu().numpy(), want)
+
+
+def test_rows_before_position_0_in_both_calls(tt):
+    """A lane with more new rows than positions is no error: the append leaves the first ones out,
+    the attention gives 0 for them; a span below 0 is reported by both."""
+    starts, spans, table, k, v = ck.batch(82, [6, 3], [0, 5], 1, 8)
+    spans[0] = 4
+    g = torch.Generator(device="cuda").manual_seed(83)
+    x = torch.randn(9, 4 * 128, device="cuda", generator=g)
+    cos, sin = (dev(t) for t in ck.tables(30, 128))
+    kd, vd, sd, pd = dev(k), dev(v), dev(starts), dev(spans)
+    kv = tt.attn.paged_cache(kd, vd, dev(table))
+    q = torch.full((9, 2, 128), 5.0, device="cuda", dtype=torch.float16)
+    tt.qkrope.rotary_append(x, 2, sd, pd, cos, sin, kv, out=q)
+    o = tt.attn.chunk_attention(q, sd, pd, kv, SCALE)
+    tt.check()
+    assert (q[:2] == 5).all() and not (q[2:] == 5).all(-1).any() and (o[:2] == 0).all()
+    # rows 2 .. 5 are at positions 0 .. 3: as four rows of their own
+    k2, v2 = dev(k), dev(v)
+    kv2 = tt.attn.paged_cache(k2, v2, dev(table))
+    q2 = tt.qkrope.rotary_append(x[2:], 2, sd.sub(2).clamp(min=0), pd, cos, sin, kv2)
+    assert torch.equal(q2, q[2:]) and torch.equal(k2, kd) and torch.equal(v2, vd)
+    assert torch.equal(tt.attn.chunk_attention(q2, sd.sub(2).clamp(min=0), pd, kv2, SCALE), o[2:])
+    tt.check()
+    bad = pd.clone()
+    bad[0] = -1
+    for call in (lambda: tt.qkrope.rotary_append(x, 2, sd, bad, cos, sin, kv),
+                 lambda: tt.attn.chunk_attention(q, sd, bad, kv, SCALE)):
+        call()
+        with pytest.raises(tt.TtsError, match="out of range"):
+            tt.check()
