@@ -668,6 +668,12 @@ static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   return x < y + nb && y < x + na;
 }
 
+// Whether `n` bytes at p share any with the cache's pools.
+static bool in_pools(const void* p, size_t n, const tts_kv_cache* kv) {
+  const size_t pool = size_t(kv->num_blocks) * kv->n_kv * kv->block_size * 256;
+  return overlap(p, n, kv->k_pages, pool) || overlap(p, n, kv->v_pages, pool);
+}
+
 static tts_status rotary_ok(const char* op, int hd, int rope_len, int rotary, int interleaved,
                             const float* cos_t, const float* sin_t) {
   const std::string name = std::string(op) + ": ";
@@ -738,6 +744,9 @@ tts_status tts_rotary_append(tts_ctx* c, const void* qkv, int qkv_f16, int heads
   if (overlap(qkv, row * (heads + 2 * size_t(kv->n_kv)) * (qkv_f16 ? 2 : 4), q_out,
               row * heads * (q_f16 ? 2 : 4)))
     return fail(TTS_ERR_INVALID_ARG, "rotary_append: q must lie apart from qkv");
+  if (in_pools(qkv, row * (heads + 2 * size_t(kv->n_kv)) * (qkv_f16 ? 2 : 4), kv) ||
+      in_pools(q_out, row * heads * (q_f16 ? 2 : 4), kv))
+    return fail(TTS_ERR_INVALID_ARG, "rotary_append: qkv and q must lie apart from the pools");
   DeviceGuard g(c->device);
   RotaryAppendRequest r;
   r.x = qkv;
@@ -794,6 +803,12 @@ tts_status tts_chunk_attention(tts_ctx* c, const void* q, int q_f16, int gqa,
   const size_t elems = size_t(b->rows) * kv->n_kv * gqa * 128;
   if (overlap(q, elems * (q_f16 ? 2 : 4), out_f16, elems * 2))
     return fail(TTS_ERR_INVALID_ARG, "chunk_attention: out must lie apart from q");
+  const size_t work = chunk_attn_workspace(c->device);
+  if (in_pools(out_f16, elems * 2, kv) || in_pools(workspace, work, kv) ||
+      overlap(workspace, work, out_f16, elems * 2) ||
+      overlap(workspace, work, q, elems * (q_f16 ? 2 : 4)))
+    return fail(TTS_ERR_INVALID_ARG,
+                "chunk_attention: out, workspace, pools and q must lie apart from one another");
   DeviceGuard g(c->device);
   ChunkAttnRequest r;
   r.q = q;

@@ -284,7 +284,7 @@ TTS_API tts_status tts_rotary(tts_ctx* ctx, const void* x, int x_f16, int rows, 
 /* tts_qk_rope_append for a ragged chunk: qkv f32 or f16 [rows][(heads + 2 n_kv) * 128]; the
  * QK-norm when `norms` is given (f32 [2][128], q's then k's weight, over the whole head), then
  * the rotation of tts_rotary at each row's position; q f32 or f16 [rows][heads][128] out (apart
- * from qkv), K and V (f16) into the pages (any page size). A position behind the tables or a
+ * from qkv and the pools), K and V (f16) into the pages (any page size). A position behind the tables or a
  * page outside the pool skips its row and is reported by tts_ctx_check; rows that are skipped, those
  * before position 0 too, leave q as it is. */
 TTS_API tts_status tts_rotary_append(tts_ctx* ctx, const void* qkv, int qkv_f16, int heads,
@@ -295,7 +295,8 @@ TTS_API tts_status tts_rotary_append(tts_ctx* ctx, const void* qkv, int qkv_f16,
 
 /* Attention of a ragged chunk over its lanes' pages, its own K and V rows included: the row at
  * position p sees positions max(0, p + 1 - window) .. p (window 0: 0 .. p), scores q.k * scale.
- * q f32 or f16 [rows][n_kv * gqa][128], out f16 of the same shape (apart from q); gqa 1..16;
+ * q f32 or f16 [rows][n_kv * gqa][128], out f16 of the same shape (apart from q, the pools and the
+ * workspace); gqa 1..16;
  * block_size a multiple of 8 unless max_blocks == 1. A row that sees no position (more new rows
  * than spans says) is 0, and what the pages hold at positions a row does not see never reaches it.
  * Pages outside the pool read as zero and are reported by tts_ctx_check. `workspace` (device,

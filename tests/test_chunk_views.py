@@ -147,3 +147,33 @@ def test_strides_of_one_row_or_head_say_nothing(monkeypatch, calls):
     got = held(monkeypatch, "tts_rotary", lambda a: (a[6], a[14]))
     qkrope.rotary(x, torch.zeros(5, dtype=torch.int32), cos, sin)
     assert got == [(144, 16)]
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import build
+    build.build()
+    return L.load()
+
+
+@pytest.mark.parametrize("which", ["k_pages", "v_pages"])
+def test_outputs_inside_the_pools_are_refused(lib, which):
+    """No GPU call is made: addresses far apart, then one buffer's end or start inside a pool."""
+    ctx = C.cast(C.create_string_buffer(256), C.c_void_p)
+    pool, page_bytes = 1 << 30, 8 * 2 * 16 * 256  # 8 pages of 2 kv heads, 16 positions
+    kv = L.KvCache(1 << 40, 1 << 41, 4096, 4, 16, 8, 2, 128)
+    setattr(kv, which, pool)
+    b = L.ChunkBatch(2, 8, 4096, 4096)
+    q, out, work, size = 1 << 33, 1 << 34, 1 << 35, 1 << 40
+    chunk = lambda q, out, work: lib.tts_chunk_attention(ctx, q, 1, 2, C.byref(b), C.byref(kv), 1.0, 0, out, work,
+                                                         size, None)
+    append = lambda x, q: lib.tts_rotary_append(ctx, x, 0, 4, C.byref(b), None, 1e-6, 4096, 4096, 64, 64, 0,
+                                                C.byref(kv), q, 0, None)
+    rows = 8 * 4 * 128  # elements of q
+    for call in (lambda: chunk(q, pool, work), lambda: chunk(q, pool - rows * 2 + 16, work),
+                 lambda: chunk(q, pool + page_bytes - 16, work), lambda: chunk(q, out, pool - 16),
+                 lambda: chunk(q, out, out - 64), lambda: chunk(q, out, q + rows * 2 - 16)):
+        assert call() == 1 and "apart from one another" in L.last_error()
+    for call in (lambda: append(pool + 16, q), lambda: append(pool - 16, q), lambda: append(q, pool + page_bytes - 16),
+                 lambda: append(q, pool - rows * 4 + 16)):
+        assert call() == 1 and "apart from the pools" in L.last_error()
