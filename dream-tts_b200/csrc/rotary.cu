@@ -128,7 +128,7 @@ struct RotaryArgs {
   const int* positions;
   const float* cos_t;
   const float* sin_t;
-  int rope_len, rotary, interleaved;
+  int rope_len, rotary;
   int* err;
 };
 
@@ -291,8 +291,8 @@ cudaError_t launch_rotary(const void* x, bool f16, int rows, int heads, int hd, 
                           const int* positions, const float* cos_t, const float* sin_t,
                           int rope_len, int rotary, bool interleaved, void* y, int ldy, int* err,
                           cudaStream_t st) {
-  RotaryArgs a{x,     y,     rows,     heads,  hd,          ldx, ldy, positions,
-               cos_t, sin_t, rope_len, rotary, interleaved, err};
+  RotaryArgs a{x,   y,         rows,  heads, hd,       ldx,
+               ldy, positions, cos_t, sin_t, rope_len, rotary, err};
   // rows a CTA: enough to give each thread an item, at most 8 (12345 rows of 20 f16 heads of 96: 8
   // rows 21.5 us, one row 36.6)
   const int at_once = f16 ? kRotHeads<__half> : kRotHeads<float>;

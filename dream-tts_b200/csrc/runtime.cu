@@ -557,7 +557,6 @@ tts_status tts_decode_attention_static_check(void* stream) {
     std::string what;
     if (code & kFlagSpanRange) what += " a span outside 1..max_span or the block table;";
     if (code & kFlagPageRange) what += " a block-table page outside the pool;";
-    if (code & kFlagChunkStarts) what += " chunk row starts that descend or leave the rows;";
     return fail(TTS_ERR_INVALID_ARG, "decode_attention_static: device data out of range (code " +
                                          std::to_string(code) + "):" + what +
                                          " those positions were clamped or read as zero");
