@@ -181,7 +181,7 @@ struct CaSmem {
   // written again four runs later, when all warps have left it)
   uint8_t q_exp[kParts - 1 ? 2 : 1][128], few_exp[kCaSegs][32];
   uint32_t tmem;
-  uint32_t repaired;  // goes up with every row that was looked at again
+  int patience;  // the waits' bound (ca_wait)
 };
 
 template <int N>
@@ -239,25 +239,20 @@ TTS_DEV float ex2(float x) {
   return y;
 }
 
-// mbar_wait_warp with its bound (about 2 s) on the SM's own clock: the softmax and the MMAs hand
-// over to each other several times a unit, and reading the global timer on each hand-over cost more
-// than the hand-over. The bound starts anew while rows are being summed again (ca_repair, which ends
-// by itself), as that may take any time at long contexts.
+// mbar_wait_warp with its bound on the SM's own clock: the softmax and the MMAs hand over to each
+// other several times a unit, and reading the global timer on each hand-over cost more than the
+// hand-over. The bound is S.patience times 2^32 clocks (about 2 s): 1, and more while rows are summed
+// again (ca_repair, which ends by itself), as that may take any time at long contexts. (Kept as one
+// word and one comparison: waits that looked for such rows' progress themselves took 448 single
+// rows over 300 positions from 181 us to 198.)
 template <typename Smem>
-TTS_DEV bool ca_wait(Smem& S, uint64_t* bar, uint32_t parity, long long limit = 4000000000ll) {
+TTS_DEV bool ca_wait(Smem& S, uint64_t* bar, uint32_t parity) {
   bool ok = mbar_try_wait(bar, parity);
   if (!ok) {
-    long long t0 = clock64();
-    uint32_t repaired = 0;  // (one bound more at first, where rows were before)
+    const long long t0 = clock64();
     do {
       ok = mbar_try_wait(bar, parity);
-      if (!ok && clock64() - t0 >= limit) {
-        const uint32_t now = *static_cast<volatile uint32_t*>(&S.repaired);
-        if (now == repaired) break;
-        repaired = now;
-        t0 = clock64();
-      }
-    } while (!ok);
+    } while (!ok && (clock64() - t0) >> 32 < *static_cast<volatile int*>(&S.patience));
   }
   return __all_sync(0xffffffffu, ok);
 }
@@ -460,7 +455,7 @@ TTS_DEV void ca_load8(const __half* p, float* x) {
 // 4 lane .. + 3 of the result to each warp lane). Never reached by finite caches. Half a warp takes
 // a position, 16 positions' rows are on their way at once: a tile of such rows over a long cache
 // should not keep the CTA for long (37 lanes of 128 rows of 8 heads over 8192 positions, the last of
-// them NaN: 34 ms, one position at a time 185).
+// them NaN: 33 ms, one position at a time 185).
 template <typename TQ>
 __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, int hi, CaAim aim,
                                        float4* o) {
@@ -675,7 +670,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     }
     fence_barrier_init();
     if (wl == 0) {
-      S.repaired = 0;
+      S.patience = 1;
       tma_prefetch_desc(&tmK);
       tma_prefetch_desc(&tmV);
     }
@@ -863,7 +858,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       }
     }
     if (!ok)  // bounded: copies still on their way
-      for (int i = 0; i < ring; ++i) ca_wait(S, &S.full[base + i], phase, 200000000ll);
+      for (int i = 0; i < ring; ++i) ca_wait(S, &S.full[base + i], phase);
   } else if (warp == 9) {
     // ---- the MMAs. Tile by tile and unit by unit: O_t += P_t.V(j), then S_t = Q_t.K(j + 1) over
     // the P just read (MMAs of one thread run in the order of their issue).
@@ -970,7 +965,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     if (!ok) {  // bounded: MMAs still running
       if (elect_one()) umma_commit(&S.drain);
       __syncwarp();
-      ca_wait(S, &S.drain, 0, 200000000ll);
+      ca_wait(S, &S.drain, 0);
     }
     }
   } else {
@@ -1210,7 +1205,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         }
         unsigned again = __ballot_sync(0xffffffffu, w.live && probe != 0.f);
         const int hi = s.pos0 + min(s.n, (s.flat0 + kCaTile - 1) / a.by_gqa + 1);
+        // a bound of waits ahead of the time that the rows take, one for each that passes
+        const long long began = clock64();
+        long long granted = 0;
         while (again) {
+          if ((clock64() - began) >> 32 >= granted) {
+            ++granted;
+            if (wl == 0) atomicAdd(&S.patience, 1);
+          }
           const int src = __ffs(again) - 1;
           again &= again - 1;
           float4 y;
@@ -1221,9 +1223,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           const int sf = __shfl_sync(0xffffffffu, w.f, src);
           const int spr = __shfl_sync(0xffffffffu, w.pr, src);
           const int at = __shfl_sync(0xffffffffu, w.rh, src);
-          const bool summed = ca_repair<TQ>(a, s, sf, hi, saim, &y);
-          if (wl == 0) atomicAdd(&S.repaired, 1u);
-          if (!summed) continue;
+          if (!ca_repair<TQ>(a, s, sf, hi, saim, &y)) continue;
           __syncwarp();  // after the row's own stores
           if (whole) {
             __half2* h = reinterpret_cast<__half2*>(r.out + (size_t)at * 128 + wl * 4);
