@@ -301,3 +301,31 @@ def test_rows_before_position_0_in_both_calls(tt):
         call()
         with pytest.raises(tt.TtsError, match="out of range"):
             tt.check()
+
+
+def test_rows_and_pages_past_32_bits(tt):
+    """Rows and pages whose elements lie past 2^31 of their buffers, in both chunk calls."""
+    rows, heads, n_kv, page = 1_060_000, 16, 8, 64  # 2^31 elements: 1,048,576 rows of q, 32768 pages
+    starts, spans, table, k, v = ck.batch(84, [30, 1, 300], [100, 400, 0], n_kv, page)
+    g = torch.Generator(device="cuda").manual_seed(85)
+    first = rows - 331
+    sd, pd = dev(starts + np.int32(first)), dev(spans)
+    far = dev(table + np.int32(33000))
+    pools = [torch.empty(33000 + len(k), n_kv, page, 128, device="cuda", dtype=torch.float16) for _ in range(2)]
+    for pool, near in zip(pools, (k, v)):
+        pool[33000:].copy_(dev(near))
+    x = torch.empty(rows, (heads + 2 * n_kv) * 128, device="cuda", dtype=torch.float16)
+    x[first:].copy_(torch.randn(331, x.shape[1], device="cuda", generator=g))
+    cos, sin = (dev(t) for t in ck.tables(500, 128))
+    q = torch.empty(rows, heads, 128, device="cuda", dtype=torch.float16)
+    out = torch.empty(rows, heads * 128, device="cuda", dtype=torch.float16)
+    kv = tt.attn.paged_cache(*pools, far)
+    tt.qkrope.rotary_append(x, heads, sd, pd, cos, sin, kv, out=q)
+    tt.attn.chunk_attention(q, sd, pd, kv, SCALE, out=out)
+    tt.check()
+    kd, vd = dev(k), dev(v)
+    kv = tt.attn.paged_cache(kd, vd, dev(table))
+    want_q = tt.qkrope.rotary_append(x[first:].clone(), heads, dev(starts), pd, cos, sin, kv)
+    want = tt.attn.chunk_attention(want_q, dev(starts), pd, kv, SCALE)
+    assert torch.equal(q[first:], want_q) and torch.equal(pools[0][33000:], kd) and torch.equal(pools[1][33000:], vd)
+    assert torch.equal(out[first:], want)
