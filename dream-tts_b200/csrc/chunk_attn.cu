@@ -24,17 +24,25 @@
 // Softmax in powers of two against a reference r: w = 2^(c s - r + 8), c = scale log2 e. r is the
 // largest c s of the row's first unit and stays while the weights of 64 positions add up to no more
 // than f16 holds; only then O and the sum are brought to a new one (random scores hardly ever ask
-// for it after the first units), so no maximum is looked for in most units. Weights keep f16's 11
-// bits down to 2^-22 of r's; sums are f32.
+// for it after the first units), so no maximum is looked for in most units. Exponentials are the
+// hardware's (2^-22), sums f32.
 //
-// Measured (16 q heads, 8 kv heads): 4096 new rows over 12288 positions 430 us, 1118 TFLOP/s, 65 %
-// of a large plain product's rate: a unit of two query tiles takes about 3.9k clocks, its MMAs 2.4k
-// to 2.9k and its exponentials 2.0k (16 a clock) of them, the rest is their hand-overs. With f32
-// queries 553 us: the scores are two products. 48 single rows over 4300 positions 146 us, 5.8 TB/s,
-// 90 % of a copy: bound by HBM. 448 single rows over 300: 180 us, 3.1 TB/s, and 592 chunks of 128
-// rows 40 us: runs of one to three units are too short to hide their start and end (about 10k
-// clocks). There the fetch of instructions counts, so loops over a unit stay rolled, queries come
-// by copies in short loops and divisions are multiplications: unrolled, those two took 325 and 54.
+// Weights are f16, as the MMA takes them beside f16 values: 11 bits down to 2^-22 of r's, fewer
+// below, none below 2^-33 (the f32 sum has those whole; over N positions they are at most N 2^-33
+// of it). On N(0, 1) values results are 2.5e-4 to 2.9e-4 of their size off, where rounding the f16
+// result alone gives 2.1e-4. The weights' lower halves would ask for a third product beside the
+// two that a unit spends 2.4k of its 3.9k clocks on; the decode step's attention, which is bound
+// by HBM at any length, does keep them.
+//
+// Measured (16 q heads, 8 kv heads; B200s differ by some percent): 4096 new rows over 12288
+// positions 434 to 458 us, 1050 to 1110 TFLOP/s, 61 to 64 % of a large plain product's rate: a unit
+// of two query tiles takes about 3.9k clocks, its MMAs 2.4k to 2.9k and its exponentials 2.0k (16 a
+// clock) of them, the rest is their hand-overs. With f32 queries 550 to 578 us: the scores are two
+// products. 48 single rows over 4300 positions 146 to 156 us, 5.4 to 5.8 TB/s, 84 to 90 % of a
+// copy: bound by HBM. 448 single rows over 300: 181 to 204 us, and 74 chunks of 128 rows (592 work tiles)
+// 39 us: runs of one to three units are too short to hide their start and end (about 10k clocks).
+// There the fetch of instructions counts, so loops over a unit stay rolled, queries come by copies
+// in short loops and divisions are multiplications: unrolled, those two took 325 and 54.
 #include <cfloat>
 #include <mutex>
 
@@ -80,7 +88,8 @@ TTS_DEV uint32_t ca_sign(uint32_t two_halves, int negate) {
 // brings its largest magnitude to [2^14, 2^15), just inside f16's range; its softmax factor is
 // divided by it (ca_factor). So the pieces hold 22 bits of an element, or 2^-39 of the row's
 // largest where that is more, whatever the row's magnitude (unscaled, elements past 65504 were
-// infinite and a row near 1e-5 lost 1e-3 of its result).
+// infinite and a row near 1e-5 lost 1e-3 of its result; finding the rows' largest costs runs of f32
+// queries: 4400 rows in chunks of up to 701 take 125 us for 117, 4096 rows 551 for 543).
 TTS_DEV void ca_copy_q(uint8_t (*tile)[kCaTileBytes], const __half* q, int rh, int r0) {
   const int wl = threadIdx.x & 31, sub = wl >> 4, e = wl & 15;
 #pragma unroll 2

@@ -234,7 +234,9 @@ TTS_API tts_status tts_topk_sample(tts_ctx* ctx, const float* logits, int rows, 
  * top_k keeps the first k of them; top_p of those the shortest prefix whose weight reaches top_p
  * of theirs (at least one id); min_p of those the ids with w >= min_p; the pick is the first id
  * at which the running weight reaches the draw times the weight of what is kept (the walk of
- * tts_topk_sample). Weights and sums are held in 64 bits. out i32 [rows]: the pick, or -1 where no
+ * tts_topk_sample). A weight is held as a multiple of 2^-44 of the largest one's, sums of them are
+ * exact: a border between two ids may lie 2^-45 of the largest's weight off for each id before it.
+ * out i32 [rows]: the pick, or -1 where no
  * id can be picked. Logits of -inf or NaN are never picked; ids at +inf share the draw.
  * `how` (NULL: none of it) gives every row its own settings, f32/i32 [rows] on the device, each
  * nullable: temperature (NULL: 1; <= 0 or NaN: the largest logit's lowest id), top_k (<= 0 or
@@ -256,10 +258,10 @@ TTS_API tts_status tts_filter_sample(tts_ctx* ctx, const void* logits, int logit
  * call's row buffers (none is fine) and spans[i] the positions it holds once they are in, so row
  * j of its n sits at position spans[i] - n + j. Rows before position 0 (more new rows than spans
  * says) have no place in the cache: the append leaves them out, their attention is 0. Rows outside
- * [row_start[0], row_start[lanes]) are left as they are. row_start int32 [lanes + 1] and spans int32 [lanes] are device memory:
- * row starts that descend or leave [0, rows] void the whole call (nothing is written), both that
- * and a span below 0 or beyond the block table (its lane's rows are skipped) are reported by
- * tts_ctx_check. lanes <= 1024. No counterpart in the reference, whose Stack::forward takes one
+ * [row_start[0], row_start[lanes]) are left as they are. row_start int32 [lanes + 1] and spans int32
+ * [lanes] are device memory: row starts that descend or leave [0, rows] void the whole call (nothing
+ * is written), both that and a span below 0 or beyond the block table (its lane's rows are skipped)
+ * are reported by tts_ctx_check. lanes <= 1024. No counterpart in the reference, whose Stack::forward takes one
  * length for the whole batch (crates/qwen3tts/src/qwen3.rs:294-467). */
 typedef struct tts_chunk_batch {
   int lanes;
@@ -299,7 +301,10 @@ TTS_API tts_status tts_rotary_append(tts_ctx* ctx, const void* qkv, int qkv_f16,
  * workspace); gqa 1..16;
  * block_size a multiple of 8 unless max_blocks == 1. A row that sees no position (more new rows
  * than spans says) is 0, and what the pages hold at positions a row does not see never reaches it.
- * Pages outside the pool read as zero and are reported by tts_ctx_check. `workspace` (device,
+ * Pages outside the pool read as zero and are reported by tts_ctx_check; pages that lie wholly before
+ * every new row's window, or behind the span, are not looked at. Queries and scores may be of any
+ * finite size. The weights meet the values as f16 (11 bits; tts_decode_attention keeps 22 and can
+ * give f32 results), sums are f32. `workspace` (device,
  * tts_chunk_attention_workspace bytes for any call on the context's device, contents of no
  * meaning before or after) belongs to the call until it ends on the GPU: calls that may overlap
  * need one each. */
