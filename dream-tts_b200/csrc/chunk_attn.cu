@@ -348,6 +348,17 @@ TTS_DEV float ca_max(const uint32_t* v, float c, float ref) {
   return max3(ref, mx * c, mx * c);
 }
 
+// Two results as f16. A mean of f16 values is no larger than the largest of them, but weights are
+// rounded and their sum is not: what that takes past f16's largest is brought back to it, and only an
+// infinity of the values' own stays one.
+constexpr float kCaLargest = 65504.f;
+TTS_DEV __half2 ca_halves(float x, float y) {
+  const auto in = [](float v) {
+    return fabsf(v) > kCaLargest && fabsf(v) < 1.01f * kCaLargest ? copysignf(kCaLargest, v) : v;
+  };
+  return __floats2half2_rn(in(x), in(y));
+}
+
 // 32 columns of the warp's TMEM lanes, without the wait.
 TTS_DEV void tmem_ld32(uint32_t a, uint32_t* r) {
   asm volatile(
@@ -867,7 +878,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
       }
     }
     if (!ok)  // bounded: copies still on their way
-      for (int i = 0; i < ring; ++i) ca_wait(S, &S.full[base + i], phase);
+      for (int i = 0; i < ring; ++i) mbar_wait(&S.full[base + i], phase, 100000000ull);
   } else if (warp == 9) {
     // ---- the MMAs. Tile by tile and unit by unit: O_t += P_t.V(j), then S_t = Q_t.K(j + 1) over
     // the P just read (MMAs of one thread run in the order of their issue).
@@ -974,7 +985,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     if (!ok) {  // bounded: MMAs still running
       if (elect_one()) umma_commit(&S.drain);
       __syncwarp();
-      ca_wait(S, &S.drain, 0);
+      mbar_wait(&S.drain, 0, 100000000ull);
     }
     }
   } else {
@@ -1161,7 +1172,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         const float total = ref == -INFINITY ? 0.f : sum;  // 0: the row saw nothing
         const float inv = total == 0.f ? 0.f : 1.f / total;
         float* part = a.part_data + (size_t)(2 * blockIdx.x + (s.begins ? 1 : 0)) * kCaPartFloats;
-        float probe = 0.f;  // NaN once a value is not finite
+        float largest = 0.f;  // magnitude of O, NaN if one is
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
           uint32_t v[32];
@@ -1181,7 +1192,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             tmem_tie32(v);
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) probe = fmaf(__uint_as_float(v[e]), 0.f, probe);
+          for (int e = 0; e < 32; e += 2)
+            largest = max3(largest, fabsf(__uint_as_float(v[e])), fabsf(__uint_as_float(v[e + 1])));
           if (!w.live) continue;
           if (whole) {
 #pragma unroll
@@ -1212,7 +1224,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           part[kCaTile * 128 + w.pr] = ref;
           part[kCaTile * 129 + w.pr] = total;
         }
-        unsigned again = __ballot_sync(0xffffffffu, w.live && probe != 0.f);
+        const bool finite = largest < INFINITY;
+        if (whole && w.live && finite && largest * inv > kCaLargest) {  // see ca_halves
+          __half* to = r.out + (size_t)w.rh * 128;
+          for (int d = 0; d < 128; ++d)
+            if (__hisinf(to[d])) to[d] = __float2half(copysignf(kCaLargest, float(to[d])));
+        }
+        unsigned again = __ballot_sync(0xffffffffu, w.live && !finite);
         const int hi = s.pos0 + min(s.n, (s.flat0 + kCaTile - 1) / a.by_gqa + 1);
         // a bound of waits ahead of the time that the rows take, one for each that passes
         const long long began = clock64();
@@ -1236,8 +1254,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
           __syncwarp();  // after the row's own stores
           if (whole) {
             __half2* h = reinterpret_cast<__half2*>(r.out + (size_t)at * 128 + wl * 4);
-            h[0] = __floats2half2_rn(y.x * sinv, y.y * sinv);
-            h[1] = __floats2half2_rn(y.z * sinv, y.w * sinv);
+            h[0] = ca_halves(y.x * sinv, y.y * sinv);
+            h[1] = ca_halves(y.z * sinv, y.w * sinv);
           } else {
             reinterpret_cast<float4*>(part)[wl * kCaTile + spr] = y;
           }
@@ -1305,8 +1323,8 @@ __global__ void __launch_bounds__(kCjThreads) chunk_attn_join_kernel(const CaArg
   __half2* h = reinterpret_cast<__half2*>(y);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    h[2 * e] = __floats2half2_rn(o[e].x * inv, o[e].y * inv);
-    h[2 * e + 1] = __floats2half2_rn(o[e].z * inv, o[e].w * inv);
+    h[2 * e] = ca_halves(o[e].x * inv, o[e].y * inv);
+    h[2 * e + 1] = ca_halves(o[e].z * inv, o[e].w * inv);
   }
   uint4* dst = reinterpret_cast<uint4*>(
       a.r.out + ((size_t)((p.row0 + tok) * a.r.n_kv + p.head - tok) * a.r.gqa + f) * 128 +

@@ -329,3 +329,23 @@ def test_rows_and_pages_past_32_bits(tt):
     want = tt.attn.chunk_attention(want_q, dev(starts), pd, kv, SCALE)
     assert torch.equal(q[first:], want_q) and torch.equal(pools[0][33000:], kd) and torch.equal(pools[1][33000:], vd)
     assert torch.equal(out[first:], want)
+
+
+@pytest.mark.parametrize("q32", [False, True])
+@pytest.mark.parametrize("new,held,window", [([200, 1, 300, 2], [100, 4000, 900, 30], 0), ([150, 40], [600, 90], 70)])
+def test_values_at_f16s_largest(tt, new, held, window, q32):
+    """A mean of values of +-65504 is no larger: roundings of the weights make none infinite."""
+    b = ck.batch(86, new, held, 8, 32)
+    starts, spans, table, k, v = b
+    v[:] = np.float16(65504)
+    v[..., 1::2] *= -1
+    for seed in range(87, 91):
+        q = np.random.default_rng(seed).standard_normal((int(starts[-1]), 16, 128)) * 2
+        got = attend(tt, q.astype(np.float32 if q32 else np.float16), b, window=window)
+        tt.check()
+        off = np.abs(got - np.tile(v[0, 0, 0].astype(np.float64), 16))
+        # each weight is half a step of f16 off at most (2^-11), 2^-13 as in attention_bound
+        assert (off <= 65504 * (2.0 ** -11 + 2.0 ** -13)).all(), off.max()
+    v[table[0, 0], :, 0] = np.inf  # seen by lane 0's rows alone, where the window reaches it
+    got = attend(tt, q.astype(np.float32 if q32 else np.float16), b, window=window)
+    assert np.isfinite(got[starts[1]:]).all() and np.isfinite(got[:starts[1]]).all() == (window > 0)
