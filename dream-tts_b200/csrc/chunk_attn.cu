@@ -35,14 +35,15 @@
 // by HBM at any length, does keep them.
 //
 // Measured (16 q heads, 8 kv heads; B200s differ by some percent): 4096 new rows over 12288
-// positions 434 to 458 us, 1050 to 1110 TFLOP/s, 61 to 64 % of a large plain product's rate: a unit
+// positions 431 to 458 us, 1050 to 1120 TFLOP/s, 61 to 65 % of a large plain product's rate: a unit
 // of two query tiles takes about 3.9k clocks, its MMAs 2.4k to 2.9k and its exponentials 2.0k (16 a
 // clock) of them, the rest is their hand-overs. With f32 queries 550 to 578 us: the scores are two
 // products. 48 single rows over 4300 positions 146 to 156 us, 5.4 to 5.8 TB/s, 84 to 90 % of a
-// copy: bound by HBM. 448 single rows over 300: 181 to 204 us, and 74 chunks of 128 rows (592 work tiles)
-// 39 us: runs of one to three units are too short to hide their start and end (about 10k clocks).
-// There the fetch of instructions counts, so loops over a unit stay rolled, queries come by copies
-// in short loops and divisions are multiplications: unrolled, those two took 325 and 54.
+// copy: bound by HBM. 448 single rows over 300: 181 to 218 us, and 74 chunks of 128 rows (592 work
+// tiles) 39 to 45 us: runs of one to three units are too short to hide their start and end (about
+// 10k clocks). There the fetch of instructions counts, so loops over a unit stay rolled, queries
+// come by copies in short loops and divisions are multiplications: unrolled, those two took 325
+// and 54.
 #include <cfloat>
 #include <mutex>
 
@@ -190,7 +191,7 @@ struct CaSmem {
   // written again four runs later, when all warps have left it)
   uint8_t q_exp[kParts - 1 ? 2 : 1][128], few_exp[kCaSegs][32];
   uint32_t tmem;
-  int patience;  // the waits' bound (ca_wait)
+  uint32_t patience;  // the waits' bound (ca_wait)
 };
 
 template <int N>
@@ -248,20 +249,27 @@ TTS_DEV float ex2(float x) {
   return y;
 }
 
+// Units of 2^32 clocks (about 2 s) of the SM.
+TTS_DEV uint32_t ca_clock() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%clock_hi;" : "=r"(t));
+  return t;
+}
 // mbar_wait_warp with its bound on the SM's own clock: the softmax and the MMAs hand over to each
 // other several times a unit, and reading the global timer on each hand-over cost more than the
-// hand-over. The bound is S.patience times 2^32 clocks (about 2 s): 1, and more while rows are summed
-// again (ca_repair, which ends by itself), as that may take any time at long contexts. (Kept as one
-// word and one comparison: waits that looked for such rows' progress themselves took 448 single
-// rows over 300 positions from 181 us to 198.)
+// hand-over. The bound is S.patience to S.patience + 1 units of ca_clock: 1 to 2, and more while
+// rows are summed again (ca_repair, which ends by itself), as that may take any time at long
+// contexts. (One word and one comparison: waits that looked for such rows' progress themselves took
+// 448 single rows over 300 positions from 181 us to 198, 64-bit clocks a long prompt from 431 to
+// 437.)
 template <typename Smem>
 TTS_DEV bool ca_wait(Smem& S, uint64_t* bar, uint32_t parity) {
   bool ok = mbar_try_wait(bar, parity);
   if (!ok) {
-    const long long t0 = clock64();
+    const uint32_t t0 = ca_clock();
     do {
       ok = mbar_try_wait(bar, parity);
-    } while (!ok && (clock64() - t0) >> 32 < *static_cast<volatile int*>(&S.patience));
+    } while (!ok && ca_clock() - t0 <= *static_cast<volatile uint32_t*>(&S.patience));
   }
   return __all_sync(0xffffffffu, ok);
 }
@@ -349,8 +357,9 @@ TTS_DEV float ca_max(const uint32_t* v, float c, float ref) {
 }
 
 // Two results as f16. A mean of f16 values is no larger than the largest of them, but weights are
-// rounded and their sum is not: what that takes past f16's largest is brought back to it, and only an
-// infinity of the values' own stays one.
+// rounded and their sum is not: what that takes past f16's largest is brought back to it, and only
+// an infinity of the values' own stays one. (Sums of the rounded weights would be exact here and took
+// a long prompt from 434 us to 470.)
 constexpr float kCaLargest = 65504.f;
 TTS_DEV __half2 ca_halves(float x, float y) {
   const auto in = [](float v) {
@@ -413,8 +422,9 @@ TTS_DEV void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc
       "r"(a), "l"(b_desc), "r"(idesc), "r"(acc)
       : "memory");
 }
-// The first position that the row at `pos` sees (0 for rows before position 0). The comparison keeps
-// the difference in range: a window may be any size, a position as far below 0 as there are rows.
+// The first position that the row at `pos` sees (0 for rows before position 0). The comparison
+// keeps the difference in range: a window may be any size, a position as far below 0 as there are
+// rows.
 TTS_DEV int ca_first(int pos, int window) {
   return window > 0 && pos >= window ? pos + 1 - window : 0;
 }
@@ -474,8 +484,8 @@ TTS_DEV void ca_load8(const __half* p, float* x) {
 // held beyond what it sees and, if one is not finite, sums the row again over what it sees (dims
 // 4 lane .. + 3 of the result to each warp lane). Never reached by finite caches. Half a warp takes
 // a position, 16 positions' rows are on their way at once: a tile of such rows over a long cache
-// should not keep the CTA for long (37 lanes of 128 rows of 8 heads over 8192 positions, the last of
-// them NaN: 33 ms, one position at a time 185).
+// should not keep the CTA for long (37 lanes of 128 rows of 8 heads over 8192 positions, the last
+// of them NaN: 33 ms, one position at a time 185).
 template <typename TQ>
 __device__ __noinline__ bool ca_repair(const CaArgs& a, const CaSeg& s, int f, int hi, CaAim aim,
                                        float4* o) {
@@ -805,8 +815,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     CaSeg s;
     while (ok && (ok = next_seg(&s)) && s.units > 0) {
       const int last = min(s.n, (s.flat0 + kCaTile - 1) / a.by_gqa + 1);
-      // the tile's rows see positions lo .. hi - 1; boxes before or behind them are not loaded (their
-      // pages may be gone), and their values are zero
+      // the tile's rows see positions lo .. hi - 1; boxes before or behind them are not loaded
+      // (their pages may be gone), and their values are zero
       const int lo = ca_first(s.pos0 + s.flat0 / a.by_gqa, r.window), hi = s.pos0 + last;
       const int* table = r.block_table + (size_t)s.lane * r.max_blocks;
       const int end = min(hi, (s.unit0 + s.units) * kCaKeys);
@@ -1238,7 +1248,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         while (again) {
           if ((clock64() - began) >> 32 >= granted) {
             ++granted;
-            if (wl == 0) atomicAdd(&S.patience, 1);
+            if (wl == 0) atomicAdd(&S.patience, 1u);
           }
           const int src = __ffs(again) - 1;
           again &= again - 1;
